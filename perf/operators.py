@@ -208,7 +208,7 @@ def _prepare_append(case, gen, seed):
     rows, ctx = _lengths(case)
     dtype, starts = TYPES[case["type"]], _starts(rows)
     listed_rows, total = starts[-1], starts[-1] + case["spare"]
-    s = dict(case=case, total=total, listed_rows=listed_rows, max_rows=max(1, max(rows)))
+    s = dict(case=case, total=total, listed_rows=listed_rows)
     s.update(_prepare_cache(case, gen, rows, ctx, dtype))
     dims = (case["kv_heads"], total, case["features"])
     s["k"], s["v"] = tiled(_normal(gen, dims, dtype)), tiled(_normal(gen, dims, dtype))
@@ -373,7 +373,6 @@ def _views(iomx, s):
         h["workspace"] = _workspace(iomx, s, iomx.sdpa_packed_workspace(**h))
     elif c["op"] == "append":
         h["rows"] = _view(iomx, s["rows"], (1, s["listed_rows"]))
-        h["max_rows"] = s["max_rows"]
     elif c["op"] == "rope":
         dims = (c["heads"], c["rows"], c["features"])
         h.update(x=_view(iomx, s["x"], dims), out=_view(iomx, s["out"], dims),
