@@ -394,6 +394,107 @@ typedef struct iomx_softmax_desc {
 
 int iomx_launch_softmax(const iomx_softmax_desc* desc, iomx_stream_t stream);
 
+/* ---- packed rows ---------------------------------------------------------- */
+
+/*
+ * A step of a server: rows of S sequences of different lengths share one row axis of T
+ * rows.  None of these operations has a counterpart in the reference, whose session runs
+ * one sequence at a time (src/session.cpp:3430-3515).  The small operands below are I32
+ * views of rank two in device memory, read by the kernels when they run, so that a
+ * recorded graph can be replayed with other lengths:
+ *
+ *   starts  [1, S+1]  sequence s has the rows starts[s] <= t < starts[s+1]; rows before
+ *                     the first start and from the last one on belong to no sequence
+ *   lengths [1, S]    tokens of sequence s that its pages hold before this step
+ *   table   [S, M]    token x of sequence s lies in page table[s][x / P], row x % P; a
+ *                     page number outside [0, N) is an absent page
+ *
+ * Page pools are [N, Hkv, P, D] views (a plane is one head of one page, so a pool may be
+ * a slice of a larger tensor, and a dense cache [S, Hkv, C, D] is a pool of S pages of C
+ * rows).  No value in these operands makes a kernel leave its tensors: starts are clamped
+ * to [0, T], lengths to [0, M * P].
+ */
+
+/*
+ * Attention of a step's rows: q [Hq,T,D], k and v [Hkv,T,D] (Hq % Hkv == 0, kv head of
+ * h = h / (Hq/Hkv)), out [T,Hq*D]; out[t, h*D + d] = sum_x softmax_x(q[h,t] . k[x] /
+ * sqrt(D)) v[x,d].  The tokens x that row i of its sequence sees are the lengths[s] cached
+ * ones (none where k_pages, v_pages, table and lengths are all null: whole prompts without
+ * a cache) and, of its sequence's own rows, the rows j <= i, or, with `tree`, those whose
+ * bit is set: `tree` is a [T,W] view of U32 words, bit j % 32 of word j / 32 of row t
+ * stands for row j of the same sequence (a tree of drafted tokens: its ancestors and
+ * itself), and rows past the last bit are not seen.  Tokens in absent pages are not seen.
+ * What a row does not see has no influence on it, infinities and NaN included.
+ *
+ * BF16 and F16, any head size up to 256.  Scores, softmax statistics and sums are F32, the
+ * unnormalised probabilities are rounded to the leaf on the matrix cores, one rounding at
+ * the store.  A row that sees nothing, or only scores of -inf, is +0; one that sees a NaN
+ * or a score of +inf is NaN.  Rows of no sequence are left as they were; `max_rows` is the
+ * caller's bound on starts[s+1] - starts[s], and rows past it are left as they were too.
+ *
+ * path 0 picks the kernel: the matrix cores where D % 16 == 0, D <= 128 and P % 16 == 0,
+ * else one wave per row and head; path 1 forces the latter (tests).
+ *
+ * iomx_sdpa_packed_workspace gives the bytes and the alignment of the workspace that the
+ * launch needs for these operands ({0, 1}: none); its contents need not be kept or cleared
+ * between calls, and calls that may overlap in time need one each.
+ */
+int iomx_sdpa_packed_workspace(int dtype, const iomx_view* q, const iomx_view* k, const iomx_view* v,
+                               const iomx_view* out, const iomx_view* starts, const iomx_view* k_pages,
+                               const iomx_view* v_pages, const iomx_view* table, const iomx_view* lengths,
+                               const iomx_view* tree, uint64_t max_rows, uint64_t* bytes, uint64_t* alignment);
+int iomx_launch_sdpa_packed(int dtype, const iomx_view* q, const iomx_view* k, const iomx_view* v,
+                            const iomx_view* out, const iomx_view* starts, const iomx_view* k_pages,
+                            const iomx_view* v_pages, const iomx_view* table, const iomx_view* lengths,
+                            const iomx_view* tree, uint64_t max_rows, void* workspace,
+                            uint64_t workspace_bytes, int path, iomx_stream_t stream);
+
+/*
+ * Split-half rotary position encoding of x[H,T,D] into out (same shape, distinct storage),
+ * row t at position positions[t] of the I32 view [1,T]: iomx_launch_rope with a position
+ * for every row.  BF16, F16 and F32, D a multiple of 16 up to 512, theta in [1, FLT_MAX].
+ * The angle is formed and reduced in binary64, so that far positions keep their accuracy
+ * (iomx_launch_rope forms it in binary32, as the reference does).  A row with a negative
+ * position is left as it was.
+ */
+int iomx_launch_rope_packed(int dtype, const iomx_view* x, const iomx_view* out, const iomx_view* positions,
+                            double theta, iomx_stream_t stream);
+
+/*
+ * Writes rows of k and v [Hkv,T,D] behind what their sequences' pages hold: entry e of
+ * sequence s (starts[s] <= e < starts[s+1]) becomes token lengths[s] + e - starts[s].  The
+ * source row is rows[e] of the I32 view `rows` [1,E] (the accepted ones of a drafted tree,
+ * say; a number outside [0,T) skips its entry), or e itself where `rows` is null (E = T).
+ * Any leaf, raw bits, D a multiple of 16.  Entries whose page is absent or past the table
+ * are skipped.  Two entries that land on one slot leave either one's row there.
+ */
+int iomx_launch_cache_append_packed(int dtype, const iomx_view* k, const iomx_view* v, const iomx_view* k_pages,
+                                    const iomx_view* v_pages, const iomx_view* starts, const iomx_view* table,
+                                    const iomx_view* lengths, const iomx_view* rows, iomx_stream_t stream);
+
+/*
+ * What a vocabulary row says: logits [..,R,V] (BF16, F16 or F32; V below 2^24), all
+ * outputs F32 / I32 views of the same leading extents:
+ *
+ *   logprobs [..,R,G]      log softmax of the row at the I32 ids tokens [..,R,G]; an id
+ *                          outside [0,V) gives -inf
+ *   entropy  [..,R,1]      -sum p log p
+ *   top_ids, top_logprobs [..,R,K]   the K most likely tokens (K <= 32, K <= V), the
+ *                          largest first, of equal logits the lowest id first
+ *
+ * Any of the three groups may be null, not all.  Sums are F32.  A logit of -inf has
+ * probability 0.  A row that holds a NaN or +inf, or nothing but -inf, has no
+ * distribution: its log probabilities (of ids in range) and entropy are NaN, its top ids
+ * -1.  The workspace is as for iomx_launch_sdpa_packed.
+ */
+int iomx_token_logprobs_workspace(int dtype, const iomx_view* logits, const iomx_view* tokens,
+                                  const iomx_view* logprobs, const iomx_view* entropy, const iomx_view* top_ids,
+                                  const iomx_view* top_logprobs, uint64_t* bytes, uint64_t* alignment);
+int iomx_launch_token_logprobs(int dtype, const iomx_view* logits, const iomx_view* tokens,
+                               const iomx_view* logprobs, const iomx_view* entropy, const iomx_view* top_ids,
+                               const iomx_view* top_logprobs, void* workspace, uint64_t workspace_bytes,
+                               iomx_stream_t stream);
+
 /* ---- introspection (no counterpart in the reference) --------------------- */
 
 /* Which kernel family the last successful launch on this thread selected

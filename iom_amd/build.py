@@ -30,6 +30,9 @@ SOURCES = [
     "iomx_layer.hip",
     "iomx_linear.hip",
     "iomx_sdpa.hip",
+    "iomx_packed.hip",
+    "iomx_sdpa_packed.hip",
+    "iomx_logprobs.hip",
 ]
 # measurement and self-tests: a library of its own, so that libiomx.so exports operations and
 # runtime only

@@ -65,6 +65,8 @@ SYMBOLS = [
     "iomx_launch_cache_append", "iomx_launch_embedding", "iomx_launch_rope",
     "iomx_launch_binary", "iomx_launch_rmsnorm", "iomx_launch_silu", "iomx_launch_silu_mul", "iomx_launch_add_rmsnorm",
     "iomx_launch_copy", "iomx_launch_scatter", "iomx_launch_gather", "iomx_launch_softmax",
+    "iomx_sdpa_packed_workspace", "iomx_launch_sdpa_packed", "iomx_launch_rope_packed",
+    "iomx_launch_cache_append_packed", "iomx_token_logprobs_workspace", "iomx_launch_token_logprobs",
     "iomx_last_launch",
 ]
 
@@ -175,6 +177,13 @@ def lib() -> C.CDLL:
         l.iomx_launch_scatter.argtypes = [C.c_int, VP, P, P]
         l.iomx_launch_gather.argtypes = [C.c_int, VP, P, P]
         l.iomx_launch_softmax.argtypes = [C.POINTER(SoftmaxDesc), P]
+        U64P = C.POINTER(C.c_uint64)
+        l.iomx_sdpa_packed_workspace.argtypes = [C.c_int] + [VP] * 10 + [C.c_uint64, U64P, U64P]
+        l.iomx_launch_sdpa_packed.argtypes = [C.c_int] + [VP] * 10 + [C.c_uint64, P, C.c_uint64, C.c_int, P]
+        l.iomx_launch_rope_packed.argtypes = [C.c_int, VP, VP, VP, C.c_double, P]
+        l.iomx_launch_cache_append_packed.argtypes = [C.c_int] + [VP] * 8 + [P]
+        l.iomx_token_logprobs_workspace.argtypes = [C.c_int] + [VP] * 6 + [U64P, U64P]
+        l.iomx_launch_token_logprobs.argtypes = [C.c_int] + [VP] * 6 + [P, C.c_uint64, P]
         l.iomx_last_launch.argtypes = [C.POINTER(LaunchInfo)]
         _lib = l
     return _lib
@@ -210,15 +219,24 @@ def last_launch() -> LaunchInfo:
 class Stream:
     def __init__(self):
         self.h = C.c_void_p()
+        self.owned = True
         check(lib().iomx_stream_create(C.byref(self.h)), "stream_create")
+
+    @classmethod
+    def at(cls, handle: int) -> "Stream":
+        """A stream that another library of the process owns (its hipStream_t; 0 is the default
+        stream): work is submitted to it, close() leaves it alone."""
+        stream = cls.__new__(cls)
+        stream.h, stream.owned = C.c_void_p(handle), False
+        return stream
 
     def synchronize(self):
         check(lib().iomx_stream_synchronize(self.h), "stream_synchronize")
 
     def close(self):
-        if self.h:
+        if self.h and self.owned:
             lib().iomx_stream_destroy(self.h)
-            self.h = C.c_void_p()
+        self.h = C.c_void_p()
 
     def begin_capture(self):
         check(lib().iomx_stream_begin_capture(self.h), "begin_capture")
@@ -291,7 +309,15 @@ class Buffer:
     def __init__(self, nbytes: int):
         self.nbytes = int(nbytes)
         self.ptr = C.c_void_p()
+        self.owned = True
         check(lib().iomx_malloc(C.byref(self.ptr), max(self.nbytes, 16)), "malloc")
+
+    @classmethod
+    def at(cls, address: int, nbytes: int) -> "Buffer":
+        """Device memory that the caller owns and keeps alive; free() leaves it alone."""
+        buf = cls.__new__(cls)
+        buf.nbytes, buf.ptr, buf.owned = int(nbytes), C.c_void_p(address), False
+        return buf
 
     def upload(self, arr: np.ndarray, offset: int = 0):
         """Host array -> device, through the page-locked staging buffer (see _staging)."""
@@ -326,9 +352,9 @@ class Buffer:
         check(lib().iomx_fill_async(self.ptr, byte, self.nbytes, stream.h if stream else None), "fill")
 
     def free(self):
-        if self.ptr:
+        if self.ptr and self.owned:
             lib().iomx_free(self.ptr)
-            self.ptr = C.c_void_p()
+        self.ptr = C.c_void_p()
 
 
 def padded(n: int) -> int:
@@ -345,6 +371,12 @@ class DeviceTensor:
     leading-axis view transforms of iom::TensorView (src/tensor_view.cpp:99-256)."""
 
     def __init__(self, dtype: int, dims: Sequence[int], fill: Optional[int] = 0):
+        self._shape(dtype, dims)
+        self.buf = Buffer(self.nbytes)
+        if fill is not None:
+            self.buf.fill(fill)
+
+    def _shape(self, dtype, dims):
         self.dtype = dtype
         self.dims = tuple(int(d) for d in dims)
         lead = self.dims[:-2]
@@ -352,9 +384,15 @@ class DeviceTensor:
         self.plane_elems = padded(self.dims[-2]) * padded(self.dims[-1])
         self.bits = LEAF_BITS[dtype]
         self.nbytes = self.planes * self.plane_elems * self.bits // 8
-        self.buf = Buffer(self.nbytes)
-        if fill is not None:
-            self.buf.fill(fill)
+
+    @classmethod
+    def at(cls, address: int, dtype: int, dims: Sequence[int]) -> "DeviceTensor":
+        """Owner storage in the tiled layout (nbytes of it) in device memory that the caller owns
+        and keeps alive, 16-byte aligned: a tensor of another library, say.  free() leaves it alone."""
+        tensor = cls.__new__(cls)
+        tensor._shape(dtype, dims)
+        tensor.buf = Buffer.at(address, tensor.nbytes)
+        return tensor
 
     def view(self) -> "DeviceView":
         lead = self.dims[:-2]
@@ -596,6 +634,72 @@ def rope(x: DeviceView, out: DeviceView, a: int, theta: float, stream: Optional[
     s_, o = x.cview(), out.cview()
     return lib().iomx_launch_rope(out.dtype, C.byref(s_), C.byref(o), C.c_uint64(a), C.c_double(theta),
                                   _h(stream))
+
+
+def _refs(*views: Optional[DeviceView]):
+    """A C argument for each view; None is a null pointer."""
+    return [None if v is None else C.byref(v.cview()) for v in views]
+
+
+def _queried(call, *args):
+    nbytes, align = C.c_uint64(0), C.c_uint64(0)
+    rc = call(*args, C.byref(nbytes), C.byref(align))
+    return rc, nbytes.value, align.value
+
+
+def _workspace(buffer: Optional["Buffer"]):
+    return (buffer.ptr, buffer.nbytes) if buffer is not None else (None, 0)
+
+
+def sdpa_packed_workspace(q: DeviceView, k: DeviceView, v: DeviceView, out: DeviceView, starts: DeviceView,
+                          k_pages: Optional[DeviceView] = None, v_pages: Optional[DeviceView] = None,
+                          table: Optional[DeviceView] = None, lengths: Optional[DeviceView] = None,
+                          tree: Optional[DeviceView] = None, max_rows: Optional[int] = None):
+    """(status, bytes, alignment) of the workspace sdpa_packed needs for these operands."""
+    return _queried(lib().iomx_sdpa_packed_workspace, out.dtype,
+                    *_refs(q, k, v, out, starts, k_pages, v_pages, table, lengths, tree),
+                    q.dims[-2] if max_rows is None else max_rows)
+
+
+def sdpa_packed(q: DeviceView, k: DeviceView, v: DeviceView, out: DeviceView, starts: DeviceView,
+                k_pages: Optional[DeviceView] = None, v_pages: Optional[DeviceView] = None,
+                table: Optional[DeviceView] = None, lengths: Optional[DeviceView] = None,
+                tree: Optional[DeviceView] = None, max_rows: Optional[int] = None,
+                workspace: Optional["Buffer"] = None, path: int = 0, stream: Optional[Stream] = None) -> int:
+    """Attention of packed rows to their sequences' pages and to each other (causal, or by `tree`)."""
+    return lib().iomx_launch_sdpa_packed(out.dtype, *_refs(q, k, v, out, starts, k_pages, v_pages, table, lengths, tree),
+                                         q.dims[-2] if max_rows is None else max_rows, *_workspace(workspace),
+                                         path, _h(stream))
+
+
+def rope_packed(x: DeviceView, out: DeviceView, positions: DeviceView, theta: float,
+                stream: Optional[Stream] = None) -> int:
+    return lib().iomx_launch_rope_packed(out.dtype, *_refs(x, out, positions), theta, _h(stream))
+
+
+def cache_append_packed(k: DeviceView, v: DeviceView, k_pages: DeviceView, v_pages: DeviceView, starts: DeviceView,
+                        table: DeviceView, lengths: DeviceView, rows: Optional[DeviceView] = None,
+                        stream: Optional[Stream] = None) -> int:
+    """Packed rows (those listed in `rows`, or all) behind what their sequences' pages hold."""
+    return lib().iomx_launch_cache_append_packed(k_pages.dtype, *_refs(k, v, k_pages, v_pages, starts, table, lengths, rows),
+                                                 _h(stream))
+
+
+def token_logprobs_workspace(logits: DeviceView, tokens: Optional[DeviceView] = None,
+                             logprobs: Optional[DeviceView] = None, entropy: Optional[DeviceView] = None,
+                             top_ids: Optional[DeviceView] = None, top_logprobs: Optional[DeviceView] = None):
+    """(status, bytes, alignment) of the workspace token_logprobs needs for these operands."""
+    return _queried(lib().iomx_token_logprobs_workspace, logits.dtype,
+                    *_refs(logits, tokens, logprobs, entropy, top_ids, top_logprobs))
+
+
+def token_logprobs(logits: DeviceView, tokens: Optional[DeviceView] = None, logprobs: Optional[DeviceView] = None,
+                   entropy: Optional[DeviceView] = None, top_ids: Optional[DeviceView] = None,
+                   top_logprobs: Optional[DeviceView] = None, workspace: Optional["Buffer"] = None,
+                   stream: Optional[Stream] = None) -> int:
+    """Log probabilities of given tokens, the entropy and the most likely tokens of every row of logits."""
+    return lib().iomx_launch_token_logprobs(logits.dtype, *_refs(logits, tokens, logprobs, entropy, top_ids, top_logprobs),
+                                            *_workspace(workspace), _h(stream))
 
 
 def dense_layout(heads: int, rows: int, cols: int) -> StageLayout:
