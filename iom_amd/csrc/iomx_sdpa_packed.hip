@@ -5,6 +5,7 @@
 //   sdpa_packed_join   joins the parts of a row block whose tokens several workgroups shared out
 //   sdpa_packed_rows   one wave per row and head, any head size up to 256 and any page size
 #include <cmath>
+#include <type_traits>
 
 #include "iomx_mfma.hpp"
 #include "iomx_packed.hpp"
@@ -153,12 +154,12 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // The matrix-core kernel.
 //
 // Rows m = i * group + g (row i of the sequence, head g of the KV head's group) are the columns of
-// the matrix products: S^T = K Q^T puts into lane (q = lane % 16, kg = lane / 16) the scores of
-// tokens 4 kg + j of a tile for column q, and in that order they are the second operand of
-// O^T = V^T P^T, whose first operand ds_read_b64_tr_b16 reads out of a V tile as it lies (the
-// sixteen lanes of quarter kg supply rows 4 kg .. 4 kg + 3 and receive a column each).  So scores
-// and probabilities never leave their lane's registers, a row's statistics are one value per lane,
-// and K and V go to LDS as they lie in memory, by the direct loader.
+// the matrix products.  S^T = K Q^T leaves in a lane scores of one column for runs of four
+// consecutive tokens, and in that order they are the second operand of O^T = V^T P^T, whose first
+// operand ds_read_b64_tr_b16 reads out of a V tile as it lies (sixteen lanes supply four token rows
+// of a tile, 128 bytes, and receive a feature column each).  So scores and probabilities never leave
+// their lane's registers, a column's statistics are one value per lane, and K and V go to LDS as
+// they lie in memory, by the direct loader.
 //
 // Softmax in one pass: p = 2^(s * scale_log2 - ref), with a reference exponent per row that is moved
 // (and the sums with it) only when a score exceeds it by more than kSlack: the sums may be up to
@@ -169,30 +170,39 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // bits: they are at most 2^(kLift + kSlack), and subnormal below 2^-22 of the largest.
 //
 // Only blocks that a row does not see in full (the ends of the cached prefix, the diagonal, trees,
-// absent pages) form masks.  There V is cleared where no row may see it, and where a value left
-// is not finite the products are formed one token at a time: 0 times infinity must not reach a row
-// that does not see it.
+// absent pages) form masks.  There V is cleared where no row may see it, and a value left that is
+// not finite is taken out of the product (0 times infinity must not reach a row that does not see
+// it): two more products count, for every row and feature, the infinities of either sign that the
+// row sees, a NaN as both.
 // ---------------------------------------------------------------------------
 
 constexpr float kLowest = -3.4028234663852886e38f;
 
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
 template <int DT> struct PackedLeaf;
 template <> struct PackedLeaf<IOMX_DT_BF16> {
     static constexpr float kSlack = 8.0f, kLift = 0.0f;
-    static constexpr uint32_t kExponent = 0x7F80u;
+    static constexpr uint32_t kExponent = 0x7F80u, kOne = 0x3F80u;
     static __device__ __forceinline__ f32x4_t mfma(u32x4 a, u32x4 b, f32x4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16_t mfma(u32x4 a, u32x4 b, f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pair(float lo, float hi) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
     }
 };
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 template <> struct PackedLeaf<IOMX_DT_F16> {
     static constexpr float kSlack = 6.0f, kLift = 8.0f;
-    static constexpr uint32_t kExponent = 0x7C00u;
+    static constexpr uint32_t kExponent = 0x7C00u, kOne = 0x3C00u;
     static __device__ __forceinline__ f32x4_t mfma(u32x4 a, u32x4 b, f32x4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16_t mfma(u32x4 a, u32x4 b, f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pair(float lo, float hi) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), f16x2));
@@ -202,10 +212,63 @@ template <> struct PackedLeaf<IOMX_DT_F16> {
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t* tr_ptr_t;
 
-// column lane % 16 of rows 4 (lane / 16) .. + 3 of a 16 x 16 tile of 16-bit elements in LDS
-__device__ __forceinline__ u32x2 read_transposed(const uint8_t* tile, uint32_t lane) {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(lptr_t)(tile + lane * 8)));
+// Sixteen lanes read 128 consecutive bytes, four rows of a tile of 16-bit elements; lane i of them
+// receives column i.
+__device__ __forceinline__ u32x2 read_transposed(const uint8_t* at) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(lptr_t)at));
 }
+
+// How a lane's values lie for products of W columns, KS = ceil(D / 32).  A "pair" is two token tiles
+// (32 tokens); a lane holds kQuads runs of four tokens of it.
+template <int DT, int KS, int W> struct PackedShape;
+
+// v_mfma_f32_16x16x32: lane = column lane % 16, quarter lane / 16.
+template <int DT, int KS> struct PackedShape<DT, KS, 16> {
+    using Acc = f32x4_t;
+    static constexpr int kSteps = KS;               // of the first product, 32 features each
+    static constexpr int kScores = 2, kAccs = 2 * KS, kQuads = 2, kHalves = 1;
+    static __device__ __forceinline__ uint32_t column(uint32_t lane) { return lane & 15u; }
+    // feature tile and byte within its row that a lane supplies in step c
+    static __device__ __forceinline__ uint32_t operand_tile(int c, uint32_t lane) { return 2 * c + (lane >> 5); }
+    static __device__ __forceinline__ uint32_t operand_byte(uint32_t lane) { return ((lane >> 4) & 1u) * 16; }
+    // first operand of S^T: byte within the pair's stage, score tile t, step c
+    static __device__ __forceinline__ uint32_t k_lane(uint32_t lane) { return (lane >> 5) * kTile16 + (lane & 15u) * 32 + operand_byte(lane); }
+    static constexpr int k_at(int t, int c) { return t * KS * 1024 + c * 1024; }
+    // tile of quad u, and which run of four tokens of it
+    static constexpr int quad_tile(int u) { return u; }
+    static __device__ __forceinline__ uint32_t quad_run(int, uint32_t lane) { return lane >> 4; }
+    // first operand of O^T: 32 tokens of feature tile d
+    static __device__ __forceinline__ uint32_t v_lane(uint32_t lane) { return lane * 8; }
+    static constexpr int v_at(int d, int, int part) { return part * KS * 1024 + d * 512; }
+    static constexpr int v_quad(int, int part) { return part; }
+    // first feature of quad u of accumulator d
+    static __device__ __forceinline__ uint32_t feature(int d, int, uint32_t lane) { return 16 * d + 4 * (lane >> 4); }
+    static constexpr int kAccQuads = 1;
+    static __device__ __forceinline__ float join(float x) { x = fmaxf(x, __shfl_xor(x, 16)); return fmaxf(x, __shfl_xor(x, 32)); }
+    static __device__ __forceinline__ float add(float x) { x += __shfl_xor(x, 16); return x + __shfl_xor(x, 32); }
+};
+
+// v_mfma_f32_32x32x16: lane = column lane % 32, half lane / 32.
+template <int DT, int KS> struct PackedShape<DT, KS, 32> {
+    using Acc = f32x16_t;
+    static constexpr int kSteps = 2 * KS;           // 16 features each
+    static constexpr int kScores = 1, kAccs = KS, kQuads = 4, kHalves = 2;
+    static __device__ __forceinline__ uint32_t column(uint32_t lane) { return lane & 31u; }
+    static __device__ __forceinline__ uint32_t operand_tile(int c, uint32_t) { return c; }
+    static __device__ __forceinline__ uint32_t operand_byte(uint32_t lane) { return (lane >> 5) * 16; }
+    static __device__ __forceinline__ uint32_t k_lane(uint32_t lane) { return ((lane >> 4) & 1u) * (KS * 1024) + (lane & 15u) * 32 + operand_byte(lane); }
+    static constexpr int k_at(int, int c) { return c * 512; }
+    static constexpr int quad_tile(int u) { return u >> 1; }
+    static __device__ __forceinline__ uint32_t quad_run(int u, uint32_t lane) { return 2 * (u & 1) + (lane >> 5); }
+    // sixteen tokens (tile h) of feature tiles 2 d and 2 d + 1
+    static __device__ __forceinline__ uint32_t v_lane(uint32_t lane) { return ((lane >> 4) & 1u) * 512 + (lane >> 5) * 128 + (lane & 15u) * 8; }
+    static constexpr int v_at(int d, int h, int part) { return h * KS * 1024 + d * 1024 + part * 256; }
+    static constexpr int v_quad(int h, int part) { return 2 * h + part; }
+    static __device__ __forceinline__ uint32_t feature(int d, int u, uint32_t lane) { return 32 * d + 8 * u + 4 * (lane >> 5); }
+    static constexpr int kAccQuads = 4;
+    static __device__ __forceinline__ float join(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
+    static __device__ __forceinline__ float add(float x) { return x + __shfl_xor(x, 32); }
+};
 
 // Where the tokens of a row block lie: `prefix` tiles of the cache, then tiles of the packed rows.
 struct PackedTiles {
@@ -214,21 +277,23 @@ struct PackedTiles {
     uint32_t count;               // all tiles
 };
 
-constexpr uint32_t packed_stage_bytes(int KS, int NT) { return (uint32_t)(NT * KS * 1024); }   // of K, and of V
-
 // WQ of the four waves share out the rows of the block and read the same tokens from LDS; the
-// 4 / WQ teams of them share out the tokens.  A wave has QT columns tiles of 16 rows; NT token
-// tiles are in LDS per team and stage.
-template <int DT, int KS, int QT, int WQ>
+// 4 / WQ teams of them share out the tokens.  A wave has QT times W columns; NT token tiles are in
+// LDS per team and stage.
+template <int DT, int KS, int W, int QT, int WQ, int NT>
 __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPackedArgs a) {
     using Leaf = PackedLeaf<DT>;
-    constexpr int WK = 4 / WQ, NT = WQ == 4 ? 4 : 2, DTL = 2 * KS;
-    constexpr uint32_t BM = 16 * QT * WQ, kStage = packed_stage_bytes(KS, NT);
-    __shared__ __attribute__((aligned(1024))) uint8_t k_lds[2][WK][kStage];
-    __shared__ __attribute__((aligned(1024))) uint8_t v_lds[2][WK][kStage];
-    const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, kg = lane >> 4;
+    using Shape = PackedShape<DT, KS, W>;
+    using Acc = typename Shape::Acc;
+    constexpr int WK = 4 / WQ, DTL = 2 * KS, QUADS = Shape::kQuads;
+    constexpr uint32_t BM = W * QT * WQ, kStage = NT * KS * 1024;
+    // Two stages of K and V, variables of their own and named where they are used: the compiler then
+    // knows that a read of one need not wait for the loader's writes to the other.
+    __shared__ __attribute__((aligned(1024))) uint8_t k_even[WK][kStage], k_odd[WK][kStage];
+    __shared__ __attribute__((aligned(1024))) uint8_t v_even[WK][kStage], v_odd[WK][kStage];
+    const uint32_t lane = threadIdx.x & 63u, column = Shape::column(lane);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t team = WQ == 4 ? 0 : wave, member = WQ == 4 ? wave : 0;
+    const uint32_t team = wave / WQ, member = wave % WQ;
 
     // unit (sequence, KV head) fastest: consecutive workgroups go to different dies, a unit's row
     // blocks to the same one where the units are a multiple of eight.  Late rows, which see the most,
@@ -257,58 +322,62 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
     tiles.count = tiles.prefix + ((seq.start + own + 15) >> 4) - tiles.first;
     const uint32_t blocks = (tiles.count + NT - 1) / NT;
     const uint32_t per_split = (blocks + a.splits - 1) / a.splits;
-    const uint32_t b_begin = split * per_split + team;
-    const uint32_t b_end = (split + 1) * per_split < blocks ? (split + 1) * per_split : blocks;
+    const uint32_t b_begin = split * per_split;
+    const uint32_t b_end = b_begin + per_split < blocks ? b_begin + per_split : blocks;
 
     // this wave's columns: rows of the sequence, and the wave's range of them
-    const uint32_t m_wave = m_block + member * 16 * QT;
+    const uint32_t m_wave = m_block + member * W * QT;
     uint32_t row_of[QT];
 #pragma unroll
-    for (int q = 0; q < QT; ++q) row_of[q] = divided(m_wave + 16 * q + l16, a.group, a.div_group);
+    for (int q = 0; q < QT; ++q) row_of[q] = divided(m_wave + W * q + column, a.group, a.div_group);
     const bool idle = m_wave >= m_end;
-    const uint32_t i_first = divided(m_wave, a.group, a.div_group);
-    const uint32_t i_last = divided(m_wave + 16 * QT - 1, a.group, a.div_group);
     const uint32_t row_tiles = a.d_tiles * kTile16;
+    const bool odd = a.d_tiles < (uint32_t)DTL;
 
-    u32x4 qf[QT][KS];
+    u32x4 qf[QT][Shape::kSteps];
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-        const uint32_t m = m_wave + 16 * q + l16, t = seq.start + row_of[q];
+        const uint32_t m = m_wave + W * q + column, t = seq.start + row_of[q];
         const uint32_t head = hkv * a.group + (m - row_of[q] * a.group);
-        const uint8_t* qr = a.q + head * a.q_head + (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32 + (kg & 1u) * 16;
+        const uint8_t* qr = a.q + head * a.q_head + (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32 + Shape::operand_byte(lane);
 #pragma unroll
-        for (int c = 0; c < KS; ++c) {
-            const uint32_t tile = 2 * c + (kg >> 1);
+        for (int c = 0; c < Shape::kSteps; ++c) {
+            const uint32_t tile = Shape::operand_tile(c, lane);
             qf[q][c] = u32x4{0, 0, 0, 0};
             if (m < m_end && tile < a.d_tiles) qf[q][c] = *reinterpret_cast<const u32x4*>(qr + tile * kTile16);
         }
     }
     // with an odd number of feature tiles the last one of a token tile's stage is not loaded: it
     // meets zeros of Q and has to be finite
-    if (a.d_tiles < (uint32_t)DTL) {
-        for (uint32_t i = threadIdx.x; i < 2 * WK * NT * 32; i += 256)
-            *reinterpret_cast<u32x4*>(&k_lds[0][0][0] + (i >> 5) * (KS * 1024) + (DTL - 1) * kTile16 + (i & 31u) * 16) = u32x4{0, 0, 0, 0};
+    if (odd) {
+        for (uint32_t i = threadIdx.x; i < WK * NT * 32; i += 256) {
+            const uint32_t at = (i >> 5) * (KS * 1024) + (DTL - 1) * kTile16 + (i & 31u) * 16;
+            *reinterpret_cast<u32x4*>(&k_even[0][0] + at) = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(&k_odd[0][0] + at) = u32x4{0, 0, 0, 0};
+        }
         __syncthreads();
     }
 
-    // page numbers of a block's tiles, one per lane below NT; ~0 where there is nothing to load
-    auto block_pages = [&](uint32_t b) -> uint32_t {
+    // page numbers of a block's tiles, one per lane below NT.  The number is not looked at before the
+    // block's turn (present_of): a comparison here would wait for the load, and with it for every
+    // tile on its way to LDS.
+    auto block_pages = [&](uint32_t b) __attribute__((always_inline)) -> uint32_t {
         const uint32_t x = b * NT + lane;
-        if (lane >= NT || b >= b_end || x >= tiles.count) return ~0u;
-        if (x >= tiles.prefix) return 0u;
-        const uint32_t slot = divided(x, a.page_tiles, a.div_page_tiles);
-        const uint32_t page = (uint32_t)a.table.at(s, slot);
-        return page < a.pages ? page : ~0u;
+        if (lane >= NT || b >= b_end || x >= tiles.prefix) return 0u;
+        return (uint32_t)a.table.at(s, divided(x, a.page_tiles, a.div_page_tiles));
     };
-    const bool odd = a.d_tiles < (uint32_t)DTL;
-    // brings the tiles of block b to a stage: wave `member` of a team of four takes tile `member`
-    auto fetch = [&](uint32_t b, uint32_t pages, uint8_t* ks, uint8_t* vs) {
+    auto present_of = [&](uint32_t b, uint32_t pages) __attribute__((always_inline)) -> uint32_t {
+        const uint32_t x = b * NT + lane;
+        return (uint32_t)__ballot(lane < NT && b < b_end && x < tiles.count && (x >= tiles.prefix || pages < a.pages));
+    };
+    // brings the tiles of block b that are present to a stage: a wave of the team takes every WQ-th
+    auto fetch = [&](uint32_t b, uint32_t pages, uint32_t present, uint8_t* ks, uint8_t* vs) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < NT / WQ; ++n) {
-            const uint32_t at = member + n;
+            const uint32_t at = member + n * WQ;
             const uint32_t x = b * NT + at;
             const uint32_t page = __builtin_amdgcn_readlane(pages, at);
-            if (page == ~0u) continue;
+            if (!((present >> at) & 1u)) continue;
             const uint8_t *kt, *vt;
             if (x < tiles.prefix) {
                 const uint32_t slot = divided(x, a.page_tiles, a.div_page_tiles);
@@ -329,281 +398,370 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
         }
     };
 
-    f32x4_t acc[DTL][QT];
+    Acc acc[Shape::kAccs][QT];
     float ref[QT], sum[QT];
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
         ref[q] = kLowest;
         sum[q] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < DTL; ++d) acc[d][q] = f32x4_t{0, 0, 0, 0};
+        for (int d = 0; d < Shape::kAccs; ++d) acc[d][q] = Acc{};
     }
-    // tiles that every row of this wave sees in full
+    // tiles that every row of this wave sees in full, and the first that none of them sees
     const uint32_t whole_prefix = tiles.cached >> 4;
     const uint32_t whole_first = tiles.prefix + ((seq.start + 15) >> 4) - tiles.first;
-    const uint32_t whole_end = a.tree.base ? 0 : tiles.prefix + ((seq.start + i_first + 1) >> 4) - tiles.first;
-    const uint32_t k_lane = (kg >> 1) * kTile16 + l16 * 32 + (kg & 1u) * 16;
+    uint32_t whole_end = 0, past = ~0u;
+    if (!a.tree.base) {
+        whole_end = tiles.prefix + ((seq.start + divided(m_wave, a.group, a.div_group) + 1) >> 4) - tiles.first;
+        past = tiles.prefix + ((seq.start + divided(m_wave + W * QT - 1, a.group, a.div_group)) >> 4) + 1 - tiles.first;
+    }
+    const uint32_t k_lane = Shape::k_lane(lane), v_lane = Shape::v_lane(lane);
 
-    // Two token tiles (x, x + 1) of the stage: scores, probabilities, sums.
-    auto two_tiles = [&](uint32_t x, uint32_t present, const uint8_t* ks, const uint8_t* vs) {
-        if (idle || !present) return;
-        // the wave's rows are all before these tokens
-        if (!a.tree.base && x >= tiles.prefix && ((tiles.first + x - tiles.prefix) << 4) > seq.start + i_last) return;
-        f32x4_t sc[2][QT];
+    // scores of a pair: [column tile][score tile]
+    auto scores = [&](const uint8_t* ks, Acc (&sc)[QT][Shape::kScores]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < Shape::kScores; ++t) {
 #pragma unroll
-            for (int q = 0; q < QT; ++q) sc[t][q] = f32x4_t{0, 0, 0, 0};
+            for (int q = 0; q < QT; ++q) sc[q][t] = Acc{};
 #pragma unroll
-            for (int c = 0; c < KS; ++c) {
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + t * (KS * 1024) + c * 1024 + k_lane);
+            for (int c = 0; c < Shape::kSteps; ++c) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + Shape::k_at(t, c) + k_lane);
 #pragma unroll
-                for (int q = 0; q < QT; ++q) sc[t][q] = Leaf::mfma(kf, qf[q][c], sc[t][q]);
+                for (int q = 0; q < QT; ++q) sc[q][t] = Leaf::mfma(kf, qf[q][c], sc[q][t]);
             }
         }
-        auto whole = [&](uint32_t y) { return y < whole_prefix || (y >= whole_first && y < whole_end); };
-        const bool masked = present != 3u || !whole(x) || !whole(x + 1);
-        uint32_t seen[QT];                  // bit 4 t + j: the column sees token 4 kg + j of tile t
-        uint32_t keep[2][2];                // V words (two tokens each) that some row may see
-        if (masked) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t y = x + t;
-                uint32_t any = 0;
-                if (!((present >> t) & 1u)) {
-#pragma unroll
-                    for (int q = 0; q < QT; ++q) seen[q] = t ? seen[q] : 0u;
-                } else if (y < tiles.prefix) {
-                    const uint32_t token = y * 16 + 4 * kg;
-                    const uint32_t n = token >= tiles.cached ? 0 : tiles.cached - token < 4 ? tiles.cached - token : 4;
-                    any = (1u << n) - 1u;
-#pragma unroll
-                    for (int q = 0; q < QT; ++q) seen[q] = t ? seen[q] | any << 4 : any;
-                } else {
-                    // own rows j .. j + 3 of the sequence
-                    const int32_t j = (int32_t)((tiles.first + y - tiles.prefix) * 16 + 4 * kg) - (int32_t)seq.start;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) any |= (uint32_t)(j + i >= 0 && j + i < (int32_t)seq.rows) << i;
-#pragma unroll
-                    for (int q = 0; q < QT; ++q) {
-                        uint32_t bits = 0;
-                        if (a.tree.base) {
-                            if (any && m_wave + 16 * q + l16 < m_end) {
-                                const uint32_t row = seq.start + row_of[q];
-                                const int32_t w = j >> 5;              // -1 for the rows before the first
-                                const uint32_t lo = w >= 0 && w < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w) : 0u;
-                                const uint32_t hi = w + 1 < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w + 1) : 0u;
-                                bits = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j & 31));
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) bits |= (uint32_t)(j + i <= (int32_t)row_of[q]) << i;
-                        }
-                        bits &= any;
-                        seen[q] = t ? seen[q] | bits << 4 : bits;
-                    }
-                }
-                keep[t][0] = ((any & 1u) ? 0xFFFFu : 0u) | ((any & 2u) ? 0xFFFF0000u : 0u);
-                keep[t][1] = ((any & 4u) ? 0xFFFFu : 0u) | ((any & 8u) ? 0xFFFF0000u : 0u);
-            }
-#pragma unroll
-            for (int q = 0; q < QT; ++q)
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        sc[t][q][j] = (seen[q] >> (4 * t + j)) & 1u ? sc[t][q][j] : -__builtin_inff();
-        }
-        // scores beyond the reference move it
-        float top[QT];
-        bool beyond = false;
+    };
+    // largest score of each column over N pairs, as an exponent of two
+    auto largest = [&](auto& sc, float (&top)[QT]) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
-            top[q] = fmaxf(fmaxf(fmaxf(sc[0][q][0], sc[0][q][1]), fmaxf(sc[0][q][2], sc[0][q][3])),
-                           fmaxf(fmaxf(sc[1][q][0], sc[1][q][1]), fmaxf(sc[1][q][2], sc[1][q][3]))) * a.scale_log2;
-            beyond = beyond || top[q] > ref[q] + Leaf::kSlack;
-        }
-        if (__any(beyond)) {
+            float most = -__builtin_inff();
 #pragma unroll
-            for (int q = 0; q < QT; ++q) {
-                float r = fmaxf(top[q], __shfl_xor(top[q], 16));
-                r = fmaxf(r, __shfl_xor(r, 32));
-                r = fmaxf(r, ref[q]);
-                const float factor = __builtin_amdgcn_exp2f(ref[q] - r);
-                ref[q] = r;
-                sum[q] *= factor;
+            for (uint32_t n = 0; n < sizeof(sc) / sizeof(sc[0]); ++n)
 #pragma unroll
-                for (int d = 0; d < DTL; ++d) acc[d][q] *= factor;
-            }
+                for (int t = 0; t < Shape::kScores; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4 * QUADS / Shape::kScores; j += 2)
+                        most = fmaxf(fmaxf(most, sc[n][q][t][j]), sc[n][q][t][j + 1]);
+            top[q] = most * a.scale_log2;
         }
-        u32x4 pf[QT];
+    };
+    auto beyond = [&](float (&top)[QT]) __attribute__((always_inline)) -> bool {
+        bool any = false;
+#pragma unroll
+        for (int q = 0; q < QT; ++q) any = any || top[q] > ref[q] + Leaf::kSlack;
+        return __any(any);
+    };
+    // probabilities of a pair, as the second product takes them: words 2 u, 2 u + 1 of quad u
+    auto probabilities = [&](Acc (&sc)[QT][Shape::kScores], uint32_t (&pw)[QT][2 * QUADS]) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
             const float minus = Leaf::kLift - ref[q];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int u = 0; u < QUADS; ++u) {
+                float p[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sc[t][q][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][q][j], a.scale_log2, minus));
-                sum[q] += (sc[t][q][0] + sc[t][q][1]) + (sc[t][q][2] + sc[t][q][3]);
+                for (int j = 0; j < 4; ++j)
+                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[q][W == 16 ? u : 0][W == 16 ? j : 4 * u + j], a.scale_log2, minus));
+                sum[q] += (p[0] + p[1]) + (p[2] + p[3]);
+                pw[q][2 * u] = Leaf::pair(p[0], p[1]);
+                pw[q][2 * u + 1] = Leaf::pair(p[2], p[3]);
             }
-            pf[q] = u32x4{Leaf::pair(sc[0][q][0], sc[0][q][1]), Leaf::pair(sc[0][q][2], sc[0][q][3]),
-                          Leaf::pair(sc[1][q][0], sc[1][q][1]), Leaf::pair(sc[1][q][2], sc[1][q][3])};
         }
-        auto values = [&](int d) {
-            const u32x2 lo = read_transposed(vs + d * kTile16, lane), hi = read_transposed(vs + KS * 1024 + d * kTile16, lane);
-            return u32x4{lo.x, lo.y, hi.x, hi.y};
-        };
-        if (!masked) {
+    };
+    // V of a pair's tokens (half h of them), accumulator d, as the second product takes it
+    auto values = [&](const uint8_t* vs, int d, int h) __attribute__((always_inline)) {
+        const u32x2 lo = read_transposed(vs + Shape::v_at(d, h, 0) + v_lane), hi = read_transposed(vs + Shape::v_at(d, h, 1) + v_lane);
+        return u32x4{lo.x, lo.y, hi.x, hi.y};
+    };
+    auto words = [&](uint32_t (&w)[2 * QUADS], int h) __attribute__((always_inline)) {
+        return u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
+    };
+    // A block that every row of the wave sees in full and whose scores are below the references; false
+    // if they are not (nothing is changed then: the path with masks takes the block, and the sums,
+    // which only that path scales, keep their registers here).
+    auto whole_block = [&](const uint8_t* ks, const uint8_t* vs) __attribute__((always_inline)) -> bool {
+        Acc sc[NT / 2][QT][Shape::kScores];
 #pragma unroll
-            for (int d = 0; d < DTL; ++d) {
-                const u32x4 vf = values(d);
+        for (int n = 0; n < NT / 2; ++n) scores(ks + n * (2 * KS * 1024), sc[n]);
+        float top[QT];
+        largest(sc, top);
+        if (beyond(top)) return false;
 #pragma unroll
-                for (int q = 0; q < QT; ++q) acc[d][q] = Leaf::mfma(vf, pf[q], acc[d][q]);
-            }
-            return;
+        for (int n = 0; n < NT / 2; ++n) {
+            uint32_t pw[QT][2 * QUADS];
+            probabilities(sc[n], pw);
+#pragma unroll
+            for (int h = 0; h < Shape::kHalves; ++h)
+#pragma unroll
+                for (int d = 0; d < Shape::kAccs; ++d) {
+                    const u32x4 vf = values(vs + n * (2 * KS * 1024), d, h);
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) acc[d][q] = Leaf::mfma(vf, words(pw[q], h), acc[d][q]);
+                }
         }
-        auto kept = [&](int d) {
-            u32x4 vf = values(d);
-            vf[0] &= keep[0][0]; vf[1] &= keep[0][1]; vf[2] &= keep[1][0]; vf[3] &= keep[1][1];
-            return vf;
-        };
-        constexpr uint32_t lo_exp = Leaf::kExponent, hi_exp = Leaf::kExponent << 16;
-        bool special = false;
+        return true;
+    };
+    // Two token tiles x, x + 1 with masks.
+    auto masked_pair = [&](uint32_t x, uint32_t present, const uint8_t* ks, const uint8_t* vs) __attribute__((always_inline)) {
+        if (!present || x >= past) return;
+        Acc sc[1][QT][Shape::kScores];
+        scores(ks, sc[0]);
+        uint32_t seen[QT];                  // bit 4 u + j: the column sees token j of quad u
+        uint32_t keep[2 * QUADS];           // V words (two tokens each) that some row may see
 #pragma unroll
-        for (int d = 0; d < DTL; ++d) {
-            if (d == DTL - 1 && odd) continue;        // not loaded, and its sums are not used
-            const u32x4 vf = kept(d);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) special = special || (vf[w] & lo_exp) == lo_exp || (vf[w] & hi_exp) == hi_exp;
-        }
-        if (!__any(special)) {
-#pragma unroll
-            for (int d = 0; d < DTL; ++d) {
-                const u32x4 vf = kept(d);
-#pragma unroll
-                for (int q = 0; q < QT; ++q) acc[d][q] = Leaf::mfma(vf, pf[q], acc[d][q]);
-            }
-            return;
-        }
-        // one token at a time: lane (q, kg) adds features 4 kg .. 4 kg + 3 of every feature tile
+        for (int q = 0; q < QT; ++q) seen[q] = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            const uint32_t y = x + t;
+            uint32_t any = 0;               // bit: token of the tile
+            uint32_t bits[QT];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-#pragma clang loop unroll(disable)
-                for (uint32_t from = 0; from < 4; ++from) {
-                    const uint8_t* vr = vs + t * (KS * 1024) + (4 * from + j) * 32 + kg * 8;
+            for (int q = 0; q < QT; ++q) bits[q] = 0;
+            if ((present >> t) & 1u) {
+                if (y < tiles.prefix) {
+                    const uint32_t left = tiles.cached - y * 16;
+                    any = left < 16 ? (1u << left) - 1u : 0xFFFFu;
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) bits[q] = any;
+                } else {
+                    // own rows j .. j + 15 of the sequence (j < 0: rows before the first)
+                    const int32_t j = (int32_t)((tiles.first + y - tiles.prefix) * 16) - (int32_t)seq.start;
+                    any = j < 0 ? 0xFFFFu << -j & 0xFFFFu : 0xFFFFu;
+                    const int32_t left = (int32_t)seq.rows - j;
+                    if (left < 16) any &= (1u << left) - 1u;
 #pragma unroll
                     for (int q = 0; q < QT; ++q) {
-                        const float p = __shfl(sc[t][q][j], from * 16 + l16);
-                        const uint32_t bits = __shfl(seen[q], from * 16 + l16);
-                        if ((bits >> (4 * t + j)) & 1u) {
-#pragma unroll
-                            for (int d = 0; d < DTL; ++d) {
-                                const u32x2 w = *reinterpret_cast<const u32x2*>(vr + d * kTile16);
-                                acc[d][q][0] = __builtin_fmaf(p, wide16<DT>(w.x & 0xFFFFu), acc[d][q][0]);
-                                acc[d][q][1] = __builtin_fmaf(p, wide16<DT>(w.x >> 16), acc[d][q][1]);
-                                acc[d][q][2] = __builtin_fmaf(p, wide16<DT>(w.y & 0xFFFFu), acc[d][q][2]);
-                                acc[d][q][3] = __builtin_fmaf(p, wide16<DT>(w.y >> 16), acc[d][q][3]);
+                        if (a.tree.base) {
+                            if (m_wave + W * q + column < m_end) {
+                                const uint32_t row = seq.start + row_of[q];
+                                const int32_t w = j >> 5;              // -1 for the rows before the first
+                                const uint32_t lo = w >= 0 && w < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w) : 0u;
+                                const uint32_t hi = w + 1 < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w + 1) : 0u;
+                                bits[q] = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j & 31)) & any;
                             }
+                        } else {
+                            const int32_t last = (int32_t)row_of[q] - j;   // the last one it sees
+                            bits[q] = (last < 0 ? 0u : last < 15 ? (2u << last) - 1u : 0xFFFFu) & any;
                         }
                     }
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < QUADS; ++u) {
+                if (Shape::quad_tile(u) != t) continue;
+                const uint32_t run = 4 * Shape::quad_run(u, lane);
+                const uint32_t k4 = any >> run;
+                keep[2 * u] = ((k4 & 1u) ? 0xFFFFu : 0u) | ((k4 & 2u) ? 0xFFFF0000u : 0u);
+                keep[2 * u + 1] = ((k4 & 4u) ? 0xFFFFu : 0u) | ((k4 & 8u) ? 0xFFFF0000u : 0u);
+#pragma unroll
+                for (int q = 0; q < QT; ++q) seen[q] |= (bits[q] >> run & 15u) << (4 * u);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+            for (int u = 0; u < QUADS; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float now = sc[0][q][W == 16 ? u : 0][W == 16 ? j : 4 * u + j];
+                    sc[0][q][W == 16 ? u : 0][W == 16 ? j : 4 * u + j] = (seen[q] >> (4 * u + j)) & 1u ? now : -__builtin_inff();
+                }
+        // scores beyond the references move them
+        float top[QT];
+        largest(sc, top);
+        if (beyond(top)) {
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+                const float r = fmaxf(Shape::join(top[q]), ref[q]);
+                const float factor = __builtin_amdgcn_exp2f(ref[q] - r);
+                ref[q] = r;
+                sum[q] *= factor;
+#pragma unroll
+                for (int d = 0; d < Shape::kAccs; ++d) acc[d][q] *= factor;
+            }
+        }
+        uint32_t pw[QT][2 * QUADS];
+        probabilities(sc[0], pw);
+#pragma unroll
+        for (int h = 0; h < Shape::kHalves; ++h) {
+#pragma unroll
+            for (int d = 0; d < Shape::kAccs; ++d) {
+                u32x4 vf = values(vs, d, h);
+                bool special = false;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    vf[w] &= keep[4 * h + w];
+                    special = special || (vf[w] & Leaf::kExponent) == Leaf::kExponent || (vf[w] >> 16 & Leaf::kExponent) == Leaf::kExponent;
+                }
+                if (__any(special)) {
+                    u32x4 plus, minus;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t up = 0, down = 0, cut = 0;
+#pragma unroll
+                        for (int half = 0; half < 32; half += 16) {
+                            const uint32_t e = vf[w] >> half & 0xFFFFu;
+                            const bool wild = (e & Leaf::kExponent) == Leaf::kExponent, nan = (e & 0x7FFFu) > Leaf::kExponent;
+                            up |= (wild && (nan || !(e & 0x8000u)) ? Leaf::kOne : 0u) << half;
+                            down |= (wild && (nan || (e & 0x8000u)) ? Leaf::kOne : 0u) << half;
+                            cut |= (wild ? 0xFFFFu : 0u) << half;
+                        }
+                        plus[w] = up;
+                        minus[w] = down;
+                        vf[w] &= ~cut;
+                    }
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) {
+                        u32x4 ones;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t two = seen[q] >> (2 * (4 * h + w));
+                            ones[w] = ((two & 1u) ? Leaf::kOne : 0u) | ((two & 2u) ? Leaf::kOne << 16 : 0u);
+                        }
+                        const Acc n = Leaf::mfma(plus, ones, Acc{}), m = Leaf::mfma(minus, ones, Acc{});
+#pragma unroll
+                        for (int j = 0; j < 4 * Shape::kAccQuads; ++j) {
+                            if (n[j] > 0.0f) acc[d][q][j] += __builtin_inff();
+                            if (m[j] > 0.0f) acc[d][q][j] -= __builtin_inff();
+                        }
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < QT; ++q) acc[d][q] = Leaf::mfma(vf, words(pw[q], h), acc[d][q]);
             }
         }
     };
 
     // Two stages: while a block is computed, the direct loader fills the other one.  The wait and
     // the barrier at the top make the block's tiles visible to the team and the other stage free.
-    uint32_t pages = block_pages(b_begin);
-    uint32_t next_pages = block_pages(b_begin + WK);
-    if (b_begin < b_end) fetch(b_begin, pages, k_lds[0][team], v_lds[0][team]);
-    auto step = [&](uint32_t b, int stage) {
-        const uint32_t present = (uint32_t)__ballot(pages != ~0u);
+    // The teams take turns at the blocks, and as many turns each.
+    uint32_t next_pages = block_pages(b_begin + team);
+    uint32_t present = present_of(b_begin + team, next_pages);
+    fetch(b_begin + team, next_pages, present, k_even[team], v_even[team]);
+    next_pages = block_pages(b_begin + team + WK);
+    auto step = [&](uint32_t b, auto stage) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x0070);        // vmcnt(0), lgkmcnt(0)
-        if constexpr (WQ == 4) __builtin_amdgcn_s_barrier();
+        if constexpr (WQ > 1) __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        pages = next_pages;
-        if (b + WK < b_end) fetch(b + WK, pages, k_lds[stage ^ 1][team], v_lds[stage ^ 1][team]);
+        const uint32_t here = present;
+        present = present_of(b + WK, next_pages);
+        if constexpr (decltype(stage)::value) fetch(b + WK, next_pages, present, k_even[team], v_even[team]);
+        else fetch(b + WK, next_pages, present, k_odd[team], v_odd[team]);
         next_pages = block_pages(b + 2 * WK);
-#pragma unroll
-        for (int h = 0; h < NT / 2; ++h)
-            two_tiles(b * NT + 2 * h, (present >> (2 * h)) & 3u, &k_lds[stage][team][h * 2 * KS * 1024],
-                      &v_lds[stage][team][h * 2 * KS * 1024]);
+        if (idle) return;
+        const uint8_t *ks, *vs;
+        if constexpr (decltype(stage)::value) { ks = &k_odd[team][0]; vs = &v_odd[team][0]; }
+        else { ks = &k_even[team][0]; vs = &v_even[team][0]; }
+        const uint32_t x = b * NT;
+        if (here == (1u << NT) - 1u && (x + NT <= whole_prefix || (x >= whole_first && x + NT <= whole_end)) && whole_block(ks, vs)) return;
+#pragma unroll 1
+        for (uint32_t n = 0; n < NT / 2; ++n)
+            masked_pair(x + 2 * n, (here >> (2 * n)) & 3u, ks + n * 2 * KS * 1024, vs + n * 2 * KS * 1024);
     };
     for (uint32_t b = b_begin; b < b_end; b += 2 * WK) {
-        step(b, 0);
+        step(b + team, std::false_type{});
         if (b + WK >= b_end) break;
-        step(b + WK, 1);
+        step(b + WK + team, std::true_type{});
     }
-    // the columns' sums over the four token quarters
+    // the columns' sums over the lanes that hold them
 #pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        sum[q] += __shfl_xor(sum[q], 16);
-        sum[q] += __shfl_xor(sum[q], 32);
-    }
+    for (int q = 0; q < QT; ++q) sum[q] = Shape::add(sum[q]);
 
-    const uint64_t part = ((uint64_t)unit * a.row_blocks + rb) * a.splits + split;
-    auto emit = [&](uint32_t m_in_block, uint32_t feature, f32x4_t o, float r, float l) {
-        const uint32_t m = m_block + m_in_block;
-        if (m >= m_end || feature >= a.D) return;
-        if (a.splits > 1) {
-            *reinterpret_cast<f32x4_t*>(a.parts + (part * BM + m_in_block) * a.D + feature) = o;
-            if (feature == 0) {
-                a.part_stats[(part * BM + m_in_block) * 2] = r;
-                a.part_stats[(part * BM + m_in_block) * 2 + 1] = l;
-            }
-            return;
-        }
-        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    // A row's place: its parts, or its first feature tile in the output (features of a head are whole
+    // tiles).
+    const uint64_t part = (((uint64_t)unit * a.row_blocks + rb) * a.splits + split) * BM;
+    auto result_of = [&](uint32_t m) __attribute__((always_inline)) -> uint8_t* {
         const uint32_t i = divided(m, a.group, a.div_group), t = seq.start + i;
-        const uint32_t col = (hkv * a.group + (m - i * a.group)) * a.D + feature;
-        u32x2 w = {narrow2<DT>(o[0] * inverse, o[1] * inverse), narrow2<DT>(o[2] * inverse, o[3] * inverse)};
-        if (l == 0.0f) w = u32x2{0, 0};
-        *reinterpret_cast<u32x2*>(a.out + ((uint64_t)(t >> 4) * a.out_tile_cols + (col >> 4)) * kTile16 + (t & 15u) * 32
-                                  + (col & 15u) * 2) = w;
+        const uint32_t head = hkv * a.group + (m - i * a.group);
+        return a.out + ((uint64_t)(t >> 4) * a.out_tile_cols + head * a.d_tiles) * kTile16 + (t & 15u) * 32;
     };
+    auto finished = [&](f32x4_t o, float l) __attribute__((always_inline)) -> u32x2 {
+        const float inverse = 1.0f / l;
+        if (l == 0.0f) return u32x2{0, 0};
+        return u32x2{narrow2<DT>(o[0] * inverse, o[1] * inverse), narrow2<DT>(o[2] * inverse, o[3] * inverse)};
+    };
+    auto quad_of = [&](const Acc& o, int u) __attribute__((always_inline)) { return f32x4_t{o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]}; };
     if constexpr (WK == 1) {
         if (idle) return;
 #pragma unroll
-        for (int q = 0; q < QT; ++q)
-#pragma unroll
-            for (int d = 0; d < DTL; ++d) emit(member * 16 * QT + 16 * q + l16, 16 * d + 4 * kg, acc[d][q], ref[q], sum[q]);
-    } else {
-        // the teams meet in LDS: a wave leaves its sums scaled to the largest reference of all
-        constexpr uint32_t kRows = 16 * QT, kFeatures = 32 * KS;
-        __shared__ float meet_ref[WK][kRows], meet_sum[WK][kRows];
-        static_assert(WK * kRows * kFeatures * 4 <= 2 * WK * kStage, "the teams' sums fit K's stages");
-        float* meet = reinterpret_cast<float*>(&k_lds[0][0][0]);     // [team][row][feature]
-        if (kg == 0) {
-#pragma unroll
-            for (int q = 0; q < QT; ++q) { meet_ref[team][16 * q + l16] = ref[q]; meet_sum[team][16 * q + l16] = sum[q]; }
-        }
-        __syncthreads();
-#pragma unroll
         for (int q = 0; q < QT; ++q) {
-            float r = kLowest;
+            const uint32_t m = m_wave + W * q + column;
+            if (m >= m_end) continue;
+            float* parts = a.splits > 1 ? a.parts + (part + m - m_block) * a.D : nullptr;
+            uint8_t* to = result_of(m);
 #pragma unroll
-            for (int w = 0; w < WK; ++w) r = fmaxf(r, meet_ref[w][16 * q + l16]);
-            const float factor = __builtin_amdgcn_exp2f(ref[q] - r);
+            for (int d = 0; d < Shape::kAccs; ++d)
 #pragma unroll
-            for (int d = 0; d < DTL; ++d)
-                *reinterpret_cast<f32x4_t*>(meet + ((team * kRows + 16 * q + l16) * kFeatures) + 16 * d + 4 * kg) = acc[d][q] * factor;
-        }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < kRows * kFeatures / 4; i += 256) {
-            const uint32_t row = i / (kFeatures / 4), feature = i % (kFeatures / 4) * 4;
-            float r = kLowest, l = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WK; ++w) r = fmaxf(r, meet_ref[w][row]);
-            f32x4_t o = {0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                l += meet_sum[w][row] * __builtin_amdgcn_exp2f(meet_ref[w][row] - r);
-                o += *reinterpret_cast<const f32x4_t*>(meet + (w * kRows + row) * kFeatures + feature);
+                for (int u = 0; u < Shape::kAccQuads; ++u) {
+                    const uint32_t feature = Shape::feature(d, u, lane);
+                    if (feature >= a.D) continue;
+                    const f32x4_t o = quad_of(acc[d][q], u);
+                    if (parts) *reinterpret_cast<f32x4_t*>(parts + feature) = o;
+                    else *reinterpret_cast<u32x2*>(to + (feature >> 4) * kTile16 + (feature & 15u) * 2) = finished(o, sum[q]);
+                }
+            if (parts && lane < W) {
+                a.part_stats[(part + m - m_block) * 2] = ref[q];
+                a.part_stats[(part + m - m_block) * 2 + 1] = sum[q];
             }
-            emit(row, feature, o, r, l);
+        }
+    } else {
+        // The teams meet in LDS, a wave's columns at a time: a wave leaves its sums scaled to the
+        // largest reference of all teams.
+        constexpr uint32_t kFeatures = 32 * KS, kRows = 16;
+        __shared__ float meet_ref[WK][BM], meet_sum[WK][BM];
+        static_assert(WK * kRows * kFeatures * 4 <= WK * kStage, "the teams' sums fit a stage of K");
+        float* meet = reinterpret_cast<float*>(&k_even[0][0]);     // [team][row][feature]
+        if (lane < W) {
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+                meet_ref[team][member * W * QT + W * q + column] = ref[q];
+                meet_sum[team][member * W * QT + W * q + column] = sum[q];
+            }
+        }
+#pragma unroll
+        for (int turn = 0; turn < (int)(BM / kRows); ++turn) {
+            __syncthreads();       // the stages, or the rows before, have been read
+            // rows turn * 16 .. of the block: sixteen columns of one column tile of one member
+            constexpr int kPerWave = W * QT / kRows;
+            if ((int)member == turn / kPerWave) {
+                const int q = (turn % kPerWave) * (int)kRows / W;
+                if (W == 16 || (int)(column >> 4) == (turn & 1)) {
+                    float r = kLowest;
+#pragma unroll
+                    for (int w = 0; w < WK; ++w) r = fmaxf(r, meet_ref[w][turn * kRows + (column & 15u)]);
+                    const float factor = __builtin_amdgcn_exp2f(ref[q] - r);
+#pragma unroll
+                    for (int d = 0; d < Shape::kAccs; ++d)
+#pragma unroll
+                        for (int u = 0; u < Shape::kAccQuads; ++u)
+                            *reinterpret_cast<f32x4_t*>(meet + (team * kRows + (column & 15u)) * kFeatures + Shape::feature(d, u, lane)) =
+                                    quad_of(acc[d][q], u) * factor;
+                }
+            }
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < kRows * kFeatures / 4; i += 256) {
+                const uint32_t row = i / (kFeatures / 4), feature = i % (kFeatures / 4) * 4, m = turn * kRows + row;
+                if (m_block + m >= m_end || feature >= a.D) continue;
+                float top = kLowest, l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) top = fmaxf(top, meet_ref[w][m]);
+                f32x4_t o = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    l += meet_sum[w][m] * __builtin_amdgcn_exp2f(meet_ref[w][m] - top);
+                    o += *reinterpret_cast<const f32x4_t*>(meet + (w * kRows + row) * kFeatures + feature);
+                }
+                if (a.splits > 1) {
+                    *reinterpret_cast<f32x4_t*>(a.parts + (part + m) * a.D + feature) = o;
+                    if (feature == 0) {
+                        a.part_stats[(part + m) * 2] = top;
+                        a.part_stats[(part + m) * 2 + 1] = l;
+                    }
+                } else
+                    *reinterpret_cast<u32x2*>(result_of(m_block + m) + (feature >> 4) * kTile16 + (feature & 15u) * 2) = finished(o, l);
+            }
         }
     }
 }
@@ -714,7 +872,7 @@ int sdpa_packed_request(int dtype, const iomx_view* q, const iomx_view* k, const
 // and the workspace their parts need.
 struct PackedPlan {
     bool mfma;
-    int tiles_per_wave;      // QT
+    int columns;             // W
     int row_waves;           // WQ
     uint32_t block_rows, row_blocks, splits;
     uint64_t parts_floats, stats_floats;
@@ -725,16 +883,14 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
     p->mfma = path != 1 && a.D % kTile == 0 && a.D <= 128 && (!a.table.base || a.page_rows % kTile == 0);
     if (!p->mfma) return IOMX_OK;
     const uint64_t m = (uint64_t)a.max_rows * a.group;       // rows of the longest sequence, per KV head
-    if (m <= 16) { p->row_waves = 1; p->tiles_per_wave = 1; }
-    else if (m <= 32) { p->row_waves = 1; p->tiles_per_wave = 2; }
-    else if (m <= 64) { p->row_waves = 4; p->tiles_per_wave = 1; }
-    else { p->row_waves = 4; p->tiles_per_wave = 2; }
-    p->block_rows = 16u * p->row_waves * p->tiles_per_wave;
+    p->columns = m <= 16 ? 16 : 32;
+    p->row_waves = m <= 32 ? 1 : m <= 64 ? 2 : 4;
+    p->block_rows = (uint32_t)(p->columns * p->row_waves);
     p->row_blocks = (uint32_t)((m + p->block_rows - 1) / p->block_rows);
     const uint64_t units = (uint64_t)a.sequences * a.Hkv, groups = units * p->row_blocks;
     // enough workgroups for two per CU; at least four blocks of tokens for each
     const uint64_t capacity = (uint64_t)a.table.cols * a.page_rows + a.max_rows;
-    const uint64_t step = p->row_waves == 4 ? 64 : 128;
+    const uint64_t step = 32 * 4 / p->row_waves;
     uint64_t splits = groups >= 512 ? 1 : 512 / groups;
     const uint64_t most = capacity / (4 * step);
     if (splits > most) splits = most;
@@ -750,14 +906,14 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
 
 template <int DT, int KS>
 void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, dim3 grid, hipStream_t st) {
-    if (p.row_waves == 1 && p.tiles_per_wave == 1)
-        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 1, 1>), grid, dim3(256), 0, st, a);
+    if (p.columns == 16)
+        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 16, 1, 1, 2>), grid, dim3(256), 0, st, a);
     else if (p.row_waves == 1)
-        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 2, 1>), grid, dim3(256), 0, st, a);
-    else if (p.tiles_per_wave == 1)
-        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 1, 4>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 32, 1, 1, 2>), grid, dim3(256), 0, st, a);
+    else if (p.row_waves == 2)
+        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 32, 1, 2, 2>), grid, dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 2, 4>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 32, 1, 4, 4>), grid, dim3(256), 0, st, a);
 }
 
 template <int DT>
