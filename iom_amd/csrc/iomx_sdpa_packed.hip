@@ -2,7 +2,7 @@
 // sees the cached tokens of its sequence (in pages) and rows of its own sequence.
 //
 //   sdpa_packed_mfma   matrix cores: a workgroup takes a block of rows of all heads of one KV head
-//   sdpa_packed_join   joins the parts of a row block whose tokens several workgroups shared out
+//   sdpa_packed_join   joins the parts of row blocks whose tokens were shared out
 //   sdpa_packed_rows   one wave per row and head, any head size up to 256 and any page size
 #include <cmath>
 #include <type_traits>
@@ -23,12 +23,12 @@ struct SdpaPackedArgs {
     FastDiv div_group, div_page_rows;
     float scale;                                              // 1 / sqrt(D)
     // the matrix-core kernel
-    uint32_t row_blocks, splits;
+    uint32_t row_blocks, shared_out;                          // tokens of a row block shared out: see PackedShare
     uint32_t page_tiles;                                      // page_rows / 16
-    FastDiv div_page_tiles, div_units, div_splits, div_hkv;
+    FastDiv div_page_tiles, div_units, div_hkv;
     float scale_log2;                                         // log2(e) / sqrt(D)
-    float* parts;                                             // [unit][row block][split][rows][D] unnormalised sums
-    float* part_stats;                                        // ... [rows][2] reference exponent and sum
+    float* parts;                                             // [workgroup][rows][D] unnormalised sums
+    float* part_stats;                                        // [workgroup][rows][2] reference exponent and sum
 };
 
 constexpr uint32_t kTile16 = 512;      // bytes of a tile of a 16-bit leaf
@@ -184,7 +184,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 template <int DT> struct PackedLeaf;
 template <> struct PackedLeaf<IOMX_DT_BF16> {
     static constexpr float kSlack = 8.0f, kLift = 0.0f;
-    static constexpr uint32_t kExponent = 0x7F80u, kOne = 0x3F80u;
+    static constexpr uint32_t kExponent = 0x7F80u, kCarry = 0x0080u, kOne = 0x3F80u;
     static __device__ __forceinline__ f32x4_t mfma(u32x4 a, u32x4 b, f32x4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     }
@@ -197,7 +197,7 @@ template <> struct PackedLeaf<IOMX_DT_BF16> {
 };
 template <> struct PackedLeaf<IOMX_DT_F16> {
     static constexpr float kSlack = 6.0f, kLift = 8.0f;
-    static constexpr uint32_t kExponent = 0x7C00u, kOne = 0x3C00u;
+    static constexpr uint32_t kExponent = 0x7C00u, kCarry = 0x0400u, kOne = 0x3C00u;
     static __device__ __forceinline__ f32x4_t mfma(u32x4 a, u32x4 b, f32x4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
     }
@@ -277,11 +277,78 @@ struct PackedTiles {
     uint32_t count;               // all tiles
 };
 
+// Where few row blocks meet long contexts, a row block's tokens are shared out among workgroups,
+// every one of which takes the same number of token blocks: the lengths are on the device, so each
+// wave adds up the work of all sequences (a sequence per lane), divides it by the workgroups the
+// launch counts on, and looks up its own piece in the running count.  A launch has a workgroup for
+// every piece of that size and one more for every row block (pieces are rounded up).
+constexpr uint32_t kPackedGroups = 512, kPackedGroupsLog2 = 9;   // workgroups to share out to
+constexpr uint32_t kPackedLeastBlocks = 4;                        // of tokens, in a piece
+
+struct PackedShare {
+    uint32_t s, row_block, piece, pieces, size;   // size: token blocks of a piece
+    uint32_t first;                               // index of the sequence's first piece (per KV head)
+};
+
+// The share of piece number `index`, or (find_sequence) of sequence `index`; s = ~0 if there is none.
+template <uint32_t BM, uint32_t NT>
+__device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uint32_t index, bool find_sequence) {
+    const uint32_t lane = threadIdx.x & 63u;
+    auto work = [&](uint32_t s, uint32_t* blocks) __attribute__((always_inline)) -> uint32_t {
+        *blocks = 0;
+        if (s >= a.sequences) return 0;
+        const PackedSequence seq = packed_sequence(a, s);
+        const uint32_t rows = seq.rows < a.max_rows ? seq.rows : a.max_rows;
+        if (!rows) return 0;
+        const uint32_t tiles = ((seq.cached + 15) >> 4) + ((seq.start + seq.rows + 15) >> 4) - (seq.start >> 4);
+        *blocks = (tiles + NT - 1) / NT;
+        return (rows * a.group + BM - 1) / BM;
+    };
+    uint32_t blocks, row_blocks = work(lane, &blocks);
+    uint64_t total = (uint64_t)row_blocks * blocks;
+    for (uint32_t s = 64 + lane; s - lane < a.sequences; s += 64) {
+        uint32_t more;
+        const uint32_t n = work(s, &more);
+        total += (uint64_t)n * more;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) total += __shfl_xor((unsigned long long)total, off);
+    PackedShare p = {};
+    const uint64_t even = (total * a.Hkv + kPackedGroups - 1) >> kPackedGroupsLog2;
+    p.size = even > kPackedLeastBlocks ? (uint32_t)even : kPackedLeastBlocks;
+    p.s = ~0u;
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
+        if (s0) row_blocks = work(s0 + lane, &blocks);
+        const uint32_t pieces = (blocks + p.size - 1) / p.size, count = row_blocks * pieces;
+        uint32_t upto = count;
+#pragma unroll
+        for (int off = 1; off < 64; off *= 2) {
+            const uint32_t lower = __shfl_up(upto, off);
+            if (lane >= (uint32_t)off) upto += lower;
+        }
+        const uint64_t here = __ballot(find_sequence ? s0 + lane == index : before + upto > index);
+        if (here) {
+            const int at = __ffsll((unsigned long long)here) - 1;
+            p.s = s0 + at;
+            p.pieces = __builtin_amdgcn_readlane(pieces, at);
+            p.first = before + __builtin_amdgcn_readlane(upto - count, at);
+            if (!find_sequence) {
+                p.row_block = (index - p.first) / p.pieces;
+                p.piece = index - p.first - p.row_block * p.pieces;
+            }
+            return p;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return p;
+}
+
 // WQ of the four waves share out the rows of the block and read the same tokens from LDS; the
 // 4 / WQ teams of them share out the tokens.  A wave has QT times W columns; NT token tiles are in
 // LDS per team and stage.
 template <int DT, int KS, int W, int QT, int WQ, int NT>
-__global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPackedArgs a) {
+__global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void sdpa_packed_mfma_kernel(const SdpaPackedArgs a) {
     using Leaf = PackedLeaf<DT>;
     using Shape = PackedShape<DT, KS, W>;
     using Acc = typename Shape::Acc;
@@ -295,14 +362,23 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t team = wave / WQ, member = wave % WQ;
 
-    // unit (sequence, KV head) fastest: consecutive workgroups go to different dies, a unit's row
-    // blocks to the same one where the units are a multiple of eight.  Late rows, which see the most,
-    // go first.
-    const uint32_t units = a.sequences * a.Hkv;
-    const uint32_t rest = divided(blockIdx.x, units, a.div_units), unit = blockIdx.x - rest * units;
-    const uint32_t rb_up = divided(rest, a.splits, a.div_splits), split = rest - rb_up * a.splits;
-    const uint32_t rb = a.row_blocks - 1 - rb_up;
-    const uint32_t s = divided(unit, a.Hkv, a.div_hkv), hkv = unit - s * a.Hkv;
+    uint32_t s, hkv, rb, piece = 0, pieces = 1, size = 0;
+    if (a.shared_out) {
+        const uint32_t index = divided(blockIdx.x, a.Hkv, a.div_hkv);
+        hkv = blockIdx.x - index * a.Hkv;
+        const PackedShare share = packed_share<BM, NT>(a, index, false);
+        if (share.s == ~0u) return;
+        s = share.s; rb = share.row_block; piece = share.piece; pieces = share.pieces; size = share.size;
+    } else {
+        // unit (sequence, KV head) fastest: consecutive workgroups go to different dies, a unit's row
+        // blocks to the same one where the units are a multiple of eight.  Late rows, which see the
+        // most, go first.
+        const uint32_t units = a.sequences * a.Hkv;
+        const uint32_t rb_up = divided(blockIdx.x, units, a.div_units), unit = blockIdx.x - rb_up * units;
+        rb = a.row_blocks - 1 - rb_up;
+        s = divided(unit, a.Hkv, a.div_hkv);
+        hkv = unit - s * a.Hkv;
+    }
     const PackedSequence seq = packed_sequence(a, s);
     const uint32_t rows = seq.rows < a.max_rows ? seq.rows : a.max_rows;
     const uint32_t m_end = rows * a.group, m_block = rb * BM;
@@ -321,9 +397,11 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
     tiles.first = seq.start >> 4;
     tiles.count = tiles.prefix + ((seq.start + own + 15) >> 4) - tiles.first;
     const uint32_t blocks = (tiles.count + NT - 1) / NT;
-    const uint32_t per_split = (blocks + a.splits - 1) / a.splits;
-    const uint32_t b_begin = split * per_split;
-    const uint32_t b_end = b_begin + per_split < blocks ? b_begin + per_split : blocks;
+    uint32_t b_begin = 0, b_end = blocks;
+    if (pieces > 1) {
+        b_begin = piece * size;
+        b_end = b_begin + size < blocks ? b_begin + size : blocks;
+    }
 
     // this wave's columns: rows of the sequence, and the wave's range of them
     const uint32_t m_wave = m_block + member * W * QT;
@@ -478,8 +556,8 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
         return u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
     };
     // A block that every row of the wave sees in full and whose scores are below the references; false
-    // if they are not (nothing is changed then: the path with masks takes the block, and the sums,
-    // which only that path scales, keep their registers here).
+    // if they are not (nothing is changed then: any_pair takes the block, and the sums, which only it
+    // scales, keep their registers here).
     auto whole_block = [&](const uint8_t* ks, const uint8_t* vs) __attribute__((always_inline)) -> bool {
         Acc sc[NT / 2][QT][Shape::kScores];
 #pragma unroll
@@ -502,71 +580,74 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
         }
         return true;
     };
-    // Two token tiles x, x + 1 with masks.
-    auto masked_pair = [&](uint32_t x, uint32_t present, const uint8_t* ks, const uint8_t* vs) __attribute__((always_inline)) {
+    // Two token tiles x, x + 1, with masks where the wave does not see both in full.
+    auto any_pair = [&](uint32_t x, uint32_t present, const uint8_t* ks, const uint8_t* vs) __attribute__((always_inline)) {
         if (!present || x >= past) return;
+        const bool whole = present == 3u && (x + 2 <= whole_prefix || (x >= whole_first && x + 2 <= whole_end));
         Acc sc[1][QT][Shape::kScores];
         scores(ks, sc[0]);
         uint32_t seen[QT];                  // bit 4 u + j: the column sees token j of quad u
         uint32_t keep[2 * QUADS];           // V words (two tokens each) that some row may see
+        if (!whole) {
 #pragma unroll
-        for (int q = 0; q < QT; ++q) seen[q] = 0;
+            for (int q = 0; q < QT; ++q) seen[q] = 0;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const uint32_t y = x + t;
-            uint32_t any = 0;               // bit: token of the tile
-            uint32_t bits[QT];
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t y = x + t;
+                uint32_t any = 0;               // bit: token of the tile
+                uint32_t bits[QT];
 #pragma unroll
-            for (int q = 0; q < QT; ++q) bits[q] = 0;
-            if ((present >> t) & 1u) {
-                if (y < tiles.prefix) {
-                    const uint32_t left = tiles.cached - y * 16;
-                    any = left < 16 ? (1u << left) - 1u : 0xFFFFu;
+                for (int q = 0; q < QT; ++q) bits[q] = 0;
+                if ((present >> t) & 1u) {
+                    if (y < tiles.prefix) {
+                        const uint32_t left = tiles.cached - y * 16;
+                        any = left < 16 ? (1u << left) - 1u : 0xFFFFu;
 #pragma unroll
-                    for (int q = 0; q < QT; ++q) bits[q] = any;
-                } else {
-                    // own rows j .. j + 15 of the sequence (j < 0: rows before the first)
-                    const int32_t j = (int32_t)((tiles.first + y - tiles.prefix) * 16) - (int32_t)seq.start;
-                    any = j < 0 ? 0xFFFFu << -j & 0xFFFFu : 0xFFFFu;
-                    const int32_t left = (int32_t)seq.rows - j;
-                    if (left < 16) any &= (1u << left) - 1u;
+                        for (int q = 0; q < QT; ++q) bits[q] = any;
+                    } else {
+                        // own rows j .. j + 15 of the sequence (j < 0: rows before the first)
+                        const int32_t j = (int32_t)((tiles.first + y - tiles.prefix) * 16) - (int32_t)seq.start;
+                        any = j < 0 ? 0xFFFFu << -j & 0xFFFFu : 0xFFFFu;
+                        const int32_t left = (int32_t)seq.rows - j;
+                        if (left < 16) any &= (1u << left) - 1u;
 #pragma unroll
-                    for (int q = 0; q < QT; ++q) {
-                        if (a.tree.base) {
-                            if (m_wave + W * q + column < m_end) {
-                                const uint32_t row = seq.start + row_of[q];
-                                const int32_t w = j >> 5;              // -1 for the rows before the first
-                                const uint32_t lo = w >= 0 && w < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w) : 0u;
-                                const uint32_t hi = w + 1 < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w + 1) : 0u;
-                                bits[q] = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j & 31)) & any;
+                        for (int q = 0; q < QT; ++q) {
+                            if (a.tree.base) {
+                                if (m_wave + W * q + column < m_end) {
+                                    const uint32_t row = seq.start + row_of[q];
+                                    const int32_t w = j >> 5;              // -1 for the rows before the first
+                                    const uint32_t lo = w >= 0 && w < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w) : 0u;
+                                    const uint32_t hi = w + 1 < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w + 1) : 0u;
+                                    bits[q] = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j & 31)) & any;
+                                }
+                            } else {
+                                const int32_t last = (int32_t)row_of[q] - j;   // the last one it sees
+                                bits[q] = (last < 0 ? 0u : last < 15 ? (2u << last) - 1u : 0xFFFFu) & any;
                             }
-                        } else {
-                            const int32_t last = (int32_t)row_of[q] - j;   // the last one it sees
-                            bits[q] = (last < 0 ? 0u : last < 15 ? (2u << last) - 1u : 0xFFFFu) & any;
                         }
                     }
                 }
-            }
 #pragma unroll
-            for (int u = 0; u < QUADS; ++u) {
-                if (Shape::quad_tile(u) != t) continue;
-                const uint32_t run = 4 * Shape::quad_run(u, lane);
-                const uint32_t k4 = any >> run;
-                keep[2 * u] = ((k4 & 1u) ? 0xFFFFu : 0u) | ((k4 & 2u) ? 0xFFFF0000u : 0u);
-                keep[2 * u + 1] = ((k4 & 4u) ? 0xFFFFu : 0u) | ((k4 & 8u) ? 0xFFFF0000u : 0u);
+                for (int u = 0; u < QUADS; ++u) {
+                    if (Shape::quad_tile(u) != t) continue;
+                    const uint32_t run = 4 * Shape::quad_run(u, lane);
+                    const uint32_t k4 = any >> run;
+                    keep[2 * u] = ((k4 & 1u) ? 0xFFFFu : 0u) | ((k4 & 2u) ? 0xFFFF0000u : 0u);
+                    keep[2 * u + 1] = ((k4 & 4u) ? 0xFFFFu : 0u) | ((k4 & 8u) ? 0xFFFF0000u : 0u);
 #pragma unroll
-                for (int q = 0; q < QT; ++q) seen[q] |= (bits[q] >> run & 15u) << (4 * u);
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < QT; ++q)
-#pragma unroll
-            for (int u = 0; u < QUADS; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float now = sc[0][q][W == 16 ? u : 0][W == 16 ? j : 4 * u + j];
-                    sc[0][q][W == 16 ? u : 0][W == 16 ? j : 4 * u + j] = (seen[q] >> (4 * u + j)) & 1u ? now : -__builtin_inff();
+                    for (int q = 0; q < QT; ++q) seen[q] |= (bits[q] >> run & 15u) << (4 * u);
                 }
+            }
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+#pragma unroll
+                for (int u = 0; u < QUADS; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float now = sc[0][q][W == 16 ? u : 0][W == 16 ? j : 4 * u + j];
+                        sc[0][q][W == 16 ? u : 0][W == 16 ? j : 4 * u + j] = (seen[q] >> (4 * u + j)) & 1u ? now : -__builtin_inff();
+                    }
+        }
         // scores beyond the references move them
         float top[QT];
         largest(sc, top);
@@ -585,32 +666,20 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
         probabilities(sc[0], pw);
 #pragma unroll
         for (int h = 0; h < Shape::kHalves; ++h) {
+            u32x4 vf[Shape::kAccs];
 #pragma unroll
-            for (int d = 0; d < Shape::kAccs; ++d) {
-                u32x4 vf = values(vs, d, h);
-                bool special = false;
+            for (int d = 0; d < Shape::kAccs; ++d) vf[d] = values(vs, d, h);
+            if (!whole) {
+                // the sign bits of `wild`: some exponent field is all ones
+                uint32_t wild = 0;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    vf[w] &= keep[4 * h + w];
-                    special = special || (vf[w] & Leaf::kExponent) == Leaf::kExponent || (vf[w] >> 16 & Leaf::kExponent) == Leaf::kExponent;
-                }
-                if (__any(special)) {
-                    u32x4 plus, minus;
+                for (int d = 0; d < Shape::kAccs; ++d)
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        uint32_t up = 0, down = 0, cut = 0;
-#pragma unroll
-                        for (int half = 0; half < 32; half += 16) {
-                            const uint32_t e = vf[w] >> half & 0xFFFFu;
-                            const bool wild = (e & Leaf::kExponent) == Leaf::kExponent, nan = (e & 0x7FFFu) > Leaf::kExponent;
-                            up |= (wild && (nan || !(e & 0x8000u)) ? Leaf::kOne : 0u) << half;
-                            down |= (wild && (nan || (e & 0x8000u)) ? Leaf::kOne : 0u) << half;
-                            cut |= (wild ? 0xFFFFu : 0u) << half;
-                        }
-                        plus[w] = up;
-                        minus[w] = down;
-                        vf[w] &= ~cut;
+                        vf[d][w] &= keep[4 * h + w];
+                        wild |= (vf[d][w] & 0x7FFF7FFFu) + (Leaf::kCarry | Leaf::kCarry << 16);
                     }
+                if (__any((wild & 0x80008000u) != 0)) {
 #pragma unroll
                     for (int q = 0; q < QT; ++q) {
                         u32x4 ones;
@@ -619,17 +688,42 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
                             const uint32_t two = seen[q] >> (2 * (4 * h + w));
                             ones[w] = ((two & 1u) ? Leaf::kOne : 0u) | ((two & 2u) ? Leaf::kOne << 16 : 0u);
                         }
-                        const Acc n = Leaf::mfma(plus, ones, Acc{}), m = Leaf::mfma(minus, ones, Acc{});
 #pragma unroll
-                        for (int j = 0; j < 4 * Shape::kAccQuads; ++j) {
-                            if (n[j] > 0.0f) acc[d][q][j] += __builtin_inff();
-                            if (m[j] > 0.0f) acc[d][q][j] -= __builtin_inff();
+                        for (int d = 0; d < Shape::kAccs; ++d) {
+                            u32x4 plus, minus;
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                uint32_t up = 0, down = 0;
+#pragma unroll
+                                for (int half = 0; half < 32; half += 16) {
+                                    const uint32_t e = vf[d][w] >> half & 0x7FFFu, negative = vf[d][w] >> half & 0x8000u;
+                                    up |= (e > Leaf::kExponent || (e == Leaf::kExponent && !negative) ? Leaf::kOne : 0u) << half;
+                                    down |= (e > Leaf::kExponent || (e == Leaf::kExponent && negative) ? Leaf::kOne : 0u) << half;
+                                }
+                                plus[w] = up;
+                                minus[w] = down;
+                            }
+                            const Acc n = Leaf::mfma(plus, ones, Acc{}), m = Leaf::mfma(minus, ones, Acc{});
+#pragma unroll
+                            for (int j = 0; j < 4 * Shape::kAccQuads; ++j) {
+                                if (n[j] > 0.0f) acc[d][q][j] += __builtin_inff();
+                                if (m[j] > 0.0f) acc[d][q][j] -= __builtin_inff();
+                            }
                         }
                     }
-                }
 #pragma unroll
-                for (int q = 0; q < QT; ++q) acc[d][q] = Leaf::mfma(vf, words(pw[q], h), acc[d][q]);
+                    for (int d = 0; d < Shape::kAccs; ++d)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t up = ((vf[d][w] & 0x7FFF7FFFu) + (Leaf::kCarry | Leaf::kCarry << 16)) & 0x80008000u;
+                            vf[d][w] &= ~(up | (up - (up >> 15)));     // both halves' bits under an all-ones exponent
+                        }
+                }
             }
+#pragma unroll
+            for (int d = 0; d < Shape::kAccs; ++d)
+#pragma unroll
+                for (int q = 0; q < QT; ++q) acc[d][q] = Leaf::mfma(vf[d], words(pw[q], h), acc[d][q]);
         }
     };
 
@@ -655,10 +749,12 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
         if constexpr (decltype(stage)::value) { ks = &k_odd[team][0]; vs = &v_odd[team][0]; }
         else { ks = &k_even[team][0]; vs = &v_even[team][0]; }
         const uint32_t x = b * NT;
-        if (here == (1u << NT) - 1u && (x + NT <= whole_prefix || (x >= whole_first && x + NT <= whole_end)) && whole_block(ks, vs)) return;
+        // (the first block sets the references)
+        if (here == (1u << NT) - 1u && (x + NT <= whole_prefix || (x >= whole_first && x + NT <= whole_end))
+            && b >= b_begin + WK && whole_block(ks, vs)) return;
 #pragma unroll 1
         for (uint32_t n = 0; n < NT / 2; ++n)
-            masked_pair(x + 2 * n, (here >> (2 * n)) & 3u, ks + n * 2 * KS * 1024, vs + n * 2 * KS * 1024);
+            any_pair(x + 2 * n, (here >> (2 * n)) & 3u, ks + n * 2 * KS * 1024, vs + n * 2 * KS * 1024);
     };
     for (uint32_t b = b_begin; b < b_end; b += 2 * WK) {
         step(b + team, std::false_type{});
@@ -671,7 +767,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
 
     // A row's place: its parts, or its first feature tile in the output (features of a head are whole
     // tiles).
-    const uint64_t part = (((uint64_t)unit * a.row_blocks + rb) * a.splits + split) * BM;
+    const uint64_t part = (uint64_t)blockIdx.x * BM;
     auto result_of = [&](uint32_t m) __attribute__((always_inline)) -> uint8_t* {
         const uint32_t i = divided(m, a.group, a.div_group), t = seq.start + i;
         const uint32_t head = hkv * a.group + (m - i * a.group);
@@ -689,7 +785,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
         for (int q = 0; q < QT; ++q) {
             const uint32_t m = m_wave + W * q + column;
             if (m >= m_end) continue;
-            float* parts = a.splits > 1 ? a.parts + (part + m - m_block) * a.D : nullptr;
+            float* parts = pieces > 1 ? a.parts + (part + m - m_block) * a.D : nullptr;
             uint8_t* to = result_of(m);
 #pragma unroll
             for (int d = 0; d < Shape::kAccs; ++d)
@@ -753,7 +849,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
                     l += meet_sum[w][m] * __builtin_amdgcn_exp2f(meet_ref[w][m] - top);
                     o += *reinterpret_cast<const f32x4_t*>(meet + (w * kRows + row) * kFeatures + feature);
                 }
-                if (a.splits > 1) {
+                if (pieces > 1) {
                     *reinterpret_cast<f32x4_t*>(a.parts + (part + m) * a.D + feature) = o;
                     if (feature == 0) {
                         a.part_stats[(part + m) * 2] = top;
@@ -766,24 +862,27 @@ __global__ __launch_bounds__(256, 2) void sdpa_packed_mfma_kernel(const SdpaPack
     }
 }
 
-// Four features of a row: the parts of its row block, each scaled from its own reference.
-template <int DT>
-__global__ __launch_bounds__(256) void sdpa_packed_join_kernel(const SdpaPackedArgs a, uint32_t block_rows) {
+// A wave joins the rows of a sequence and KV head whose tokens were shared out: a lane takes four
+// features of a row, and scales each part from its own reference.
+template <int DT, uint32_t BM, uint32_t NT>
+__global__ __launch_bounds__(256) void sdpa_packed_join_kernel(const SdpaPackedArgs a) {
     const uint32_t chunks = a.D / 4;
-    const uint32_t unit = blockIdx.y + blockIdx.z * 65535u;
-    if (unit >= a.sequences * a.Hkv) return;
-    const uint32_t s = divided(unit, a.Hkv, a.div_hkv), hkv = unit - s * a.Hkv;
+    const uint32_t s = divided(blockIdx.y, a.Hkv, a.div_hkv), hkv = blockIdx.y - s * a.Hkv;
+    const PackedShare share = packed_share<BM, NT>(a, s, true);
+    if (share.pieces <= 1) return;
     const PackedSequence seq = packed_sequence(a, s);
     const uint32_t rows = seq.rows < a.max_rows ? seq.rows : a.max_rows;
     const uint32_t at = blockIdx.x * 256 + threadIdx.x, m = at / chunks, feature = at % chunks * 4;
     if (m >= rows * a.group) return;
-    const uint64_t first = ((uint64_t)unit * a.row_blocks + m / block_rows) * a.splits * block_rows + m % block_rows;
+    // the parts are Hkv workgroups apart
+    const uint64_t first = ((uint64_t)(share.first + m / BM * share.pieces) * a.Hkv + hkv) * BM + m % BM;
+    const uint64_t step = (uint64_t)a.Hkv * BM;
     float r = kLowest;
-    for (uint32_t p = 0; p < a.splits; ++p) r = fmaxf(r, a.part_stats[(first + (uint64_t)p * block_rows) * 2]);
+    for (uint32_t p = 0; p < share.pieces; ++p) r = fmaxf(r, a.part_stats[(first + p * step) * 2]);
     float l = 0.0f;
     f32x4_t o = {0, 0, 0, 0};
-    for (uint32_t p = 0; p < a.splits; ++p) {
-        const uint64_t row = first + (uint64_t)p * block_rows;
+    for (uint32_t p = 0; p < share.pieces; ++p) {
+        const uint64_t row = first + p * step;
         const float factor = __builtin_amdgcn_exp2f(a.part_stats[row * 2] - r);
         l += a.part_stats[row * 2 + 1] * factor;
         o += *reinterpret_cast<const f32x4_t*>(a.parts + row * a.D + feature) * factor;
@@ -868,13 +967,14 @@ int sdpa_packed_request(int dtype, const iomx_view* q, const iomx_view* k, const
     return IOMX_OK;
 }
 
-// How a request runs on the matrix cores: rows of a block, workgroups that share a block's tokens,
-// and the workspace their parts need.
+// How a request runs on the matrix cores: the rows of a block, whether its tokens are shared out,
+// and the workspace the parts need.
 struct PackedPlan {
-    bool mfma;
+    bool mfma, shared_out;
     int columns;             // W
     int row_waves;           // WQ
-    uint32_t block_rows, row_blocks, splits;
+    uint32_t block_rows, row_blocks;
+    uint64_t groups;         // workgroups
     uint64_t parts_floats, stats_floats;
 };
 
@@ -887,48 +987,45 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
     p->row_waves = m <= 32 ? 1 : m <= 64 ? 2 : 4;
     p->block_rows = (uint32_t)(p->columns * p->row_waves);
     p->row_blocks = (uint32_t)((m + p->block_rows - 1) / p->block_rows);
-    const uint64_t units = (uint64_t)a.sequences * a.Hkv, groups = units * p->row_blocks;
-    // enough workgroups for two per CU; at least four blocks of tokens for each
+    p->groups = (uint64_t)a.sequences * a.Hkv * p->row_blocks;
+    // Shared out where there are fewer row blocks than two per CU and a sequence may have tokens for
+    // more than one piece.
     const uint64_t capacity = (uint64_t)a.table.cols * a.page_rows + a.max_rows;
-    const uint64_t step = 32 * 4 / p->row_waves;
-    uint64_t splits = groups >= 512 ? 1 : 512 / groups;
-    const uint64_t most = capacity / (4 * step);
-    if (splits > most) splits = most;
-    if (splits > 64) splits = 64;
-    p->splits = (uint32_t)(splits ? splits : 1);
-    if (groups * p->splits > 0x7FFFFFF0ull) return IOMX_ERR_OVERFLOW;
-    if (p->splits > 1) {
-        p->stats_floats = (groups * p->splits * p->block_rows * 2 + 63) / 64 * 64;
-        p->parts_floats = groups * p->splits * p->block_rows * a.D;
+    const uint64_t least = kPackedLeastBlocks * (p->row_waves == 4 ? 64 : 32);
+    if (p->groups < kPackedGroups && capacity > 2 * least) {
+        p->shared_out = true;
+        p->groups += (kPackedGroups + a.Hkv - 1) / a.Hkv * (uint64_t)a.Hkv;
+        p->stats_floats = (p->groups * p->block_rows * 2 + 63) / 64 * 64;
+        p->parts_floats = p->groups * p->block_rows * a.D;
     }
+    if (p->groups > 0x7FFFFFF0ull) return IOMX_ERR_OVERFLOW;
     return IOMX_OK;
 }
 
+template <int DT, int KS, int W, int WQ, int NT>
+void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, hipStream_t st) {
+    hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, W, 1, WQ, NT>), dim3((uint32_t)p.groups), dim3(256), 0, st, a);
+    if (!p.shared_out) return;
+    const uint64_t lanes = (uint64_t)a.max_rows * a.group * (a.D / 4);
+    const dim3 joins((uint32_t)((lanes + 255) / 256), a.sequences * a.Hkv);     // fewer than kPackedGroups of them
+    hipLaunchKernelGGL((sdpa_packed_join_kernel<DT, W * WQ, NT>), joins, dim3(256), 0, st, a);
+}
+
 template <int DT, int KS>
-void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, dim3 grid, hipStream_t st) {
-    if (p.columns == 16)
-        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 16, 1, 1, 2>), grid, dim3(256), 0, st, a);
-    else if (p.row_waves == 1)
-        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 32, 1, 1, 2>), grid, dim3(256), 0, st, a);
-    else if (p.row_waves == 2)
-        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 32, 1, 2, 2>), grid, dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, 32, 1, 4, 4>), grid, dim3(256), 0, st, a);
+void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, hipStream_t st) {
+    if (p.columns == 16) launch_packed<DT, KS, 16, 1, 2>(a, p, st);
+    else if (p.row_waves == 1) launch_packed<DT, KS, 32, 1, 2>(a, p, st);
+    else if (p.row_waves == 2) launch_packed<DT, KS, 32, 2, 2>(a, p, st);
+    else launch_packed<DT, KS, 32, 4, 4>(a, p, st);
 }
 
 template <int DT>
-void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, dim3 grid, hipStream_t st) {
+void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, hipStream_t st) {
     switch ((a.D + 31) / 32) {
-        case 1: launch_packed<DT, 1>(a, p, grid, st); break;
-        case 2: launch_packed<DT, 2>(a, p, grid, st); break;
-        case 3: launch_packed<DT, 3>(a, p, grid, st); break;
-        default: launch_packed<DT, 4>(a, p, grid, st); break;
-    }
-    if (p.splits > 1) {
-        const uint64_t lanes = (uint64_t)a.max_rows * a.group * (a.D / 4);
-        const uint64_t units = (uint64_t)a.sequences * a.Hkv;
-        const dim3 joins((uint32_t)((lanes + 255) / 256), (uint32_t)(units < 65535 ? units : 65535), (uint32_t)((units + 65534) / 65535));
-        hipLaunchKernelGGL(sdpa_packed_join_kernel<DT>, joins, dim3(256), 0, st, a, p.block_rows);
+        case 1: launch_packed<DT, 1>(a, p, st); break;
+        case 2: launch_packed<DT, 2>(a, p, st); break;
+        case 3: launch_packed<DT, 3>(a, p, st); break;
+        default: launch_packed<DT, 4>(a, p, st); break;
     }
 }
 
@@ -969,19 +1066,17 @@ extern "C" int iomx_launch_sdpa_packed(int dtype, const iomx_view* q, const iomx
         if (bytes && (!workspace || workspace_bytes < bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
             return IOMX_ERR_INVALID;
         a.row_blocks = p.row_blocks;
-        a.splits = p.splits;
+        a.shared_out = p.shared_out;
         a.page_tiles = a.page_rows / kTile;
         a.div_page_tiles = make_fast_div(a.page_tiles);
         a.div_units = make_fast_div(a.sequences * a.Hkv);
-        a.div_splits = make_fast_div(a.splits);
         a.div_hkv = make_fast_div(a.Hkv);
         a.scale_log2 = 1.44269504088896340736f * a.scale;
         a.part_stats = static_cast<float*>(workspace);
         a.parts = a.part_stats + p.stats_floats;
-        const dim3 grid(a.sequences * a.Hkv * p.row_blocks * p.splits);
-        if (dtype == IOMX_DT_BF16) launch_packed<IOMX_DT_BF16>(a, p, grid, st);
-        else launch_packed<IOMX_DT_F16>(a, p, grid, st);
-        record_launch(p.row_waves == 1 ? "sdpa_packed_few" : "sdpa_packed_mfma", grid.x, 256, (uint64_t)a.T * a.Hq);
+        if (dtype == IOMX_DT_BF16) launch_packed<IOMX_DT_BF16>(a, p, st);
+        else launch_packed<IOMX_DT_F16>(a, p, st);
+        record_launch(p.columns == 16 ? "sdpa_packed_few" : "sdpa_packed_mfma", (uint32_t)p.groups, 256, (uint64_t)a.T * a.Hq);
         IOMX_HIP(hipGetLastError());
         return IOMX_OK;
     }

@@ -421,6 +421,7 @@ class DeviceView:
         self.dims = tuple(int(d) for d in dims)
         self.plane_offset = int(plane_offset)
         self.plane_strides = tuple(int(s) for s in plane_strides)
+        self._held = None   # (C struct, reference to it): see ref()
 
     @property
     def dtype(self):
@@ -475,6 +476,16 @@ class DeviceView:
         for i, s in enumerate(self.plane_strides):
             v.plane_strides[i] = s
         return v
+
+    def ref(self):
+        """The view as a C argument: one struct per DeviceView, built on the first use (a struct
+        per call costs more than the rest of a small launch)."""
+        if self._held is None:
+            view = self.cview()
+            self._held = view, C.byref(view)
+        view, reference = self._held
+        view.base = self.owner.buf.ptr.value     # a freed owner is a null pointer, which is refused
+        return reference
 
     @property
     def logical_count(self) -> int:
@@ -638,7 +649,7 @@ def rope(x: DeviceView, out: DeviceView, a: int, theta: float, stream: Optional[
 
 def _refs(*views: Optional[DeviceView]):
     """A C argument for each view; None is a null pointer."""
-    return [None if v is None else C.byref(v.cview()) for v in views]
+    return [None if v is None else v.ref() for v in views]
 
 
 def _queried(call, *args):
