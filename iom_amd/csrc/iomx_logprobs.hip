@@ -17,7 +17,36 @@ struct LogprobsArgs {
     uint32_t R, V, G, K;
     uint32_t tile_cols, given_tile_cols, top_tile_cols;
     FastDiv div_rows;
+    // how the scan is laid out
+    uint32_t rows, bands;            // rows of all planes; tile rows of a plane
+    uint32_t splits, cells_per_split, cells, cell_groups, group_tiles;
+    FastDiv div_splits, div_bands;
+    float* stats;                    // [plane][tile row][split][16 rows][4]: M, sum e^d, sum d e^d
+    float* cell_max;                 // [plane][tile row][cell][16 rows], null where no top is asked for
 };
+
+// ---------------------------------------------------------------------------
+// token_logprobs_scan reads the logits once.  A band (16 rows of a plane) lies in memory as one run
+// of tiles, so a wave's loads are whole kilobytes and a lane meets one row only: lane (row, part of a
+// tile row).  It keeps the row's maximum M, sum e^d and sum d e^d with d = x - M (a difference, not a
+// product with log2 e taken from another: logits near the ends of the range stay finite), 64 or 16
+// logits at a time with the maximum moved before each, and the maximum of every cell of 256 (or 64,
+// or a multiple) columns goes to the workspace.  A few operations and one
+// exponential per logit keep the vector units at about two thirds of what the memory leaves them.
+//
+// token_logprobs_finish, one wave per row, joins the sums and picks the most likely tokens without
+// another pass: the K-th largest cell maximum bounds the K-th largest logit from below, so only the
+// cells that reach it are read again, and in them the logits that reach it are few; each counts
+// those before it (larger, or equal with a lower id), which is its place.
+// ---------------------------------------------------------------------------
+
+constexpr uint32_t kMostCells = 1024;         // of a row: sixteen per lane
+constexpr uint32_t kMostCandidates = 128;     // of a row: two per lane
+
+// d as a factor of e^d: from -200 on down e^d is 0 in F32, and its product with d is, too
+__device__ __forceinline__ float at_least(float d) { return fmaxf(d, -200.0f); }
+// e^d for d <= 0, to a few units in the last place for the d whose exponential is not tiny
+__device__ __forceinline__ float exponential(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f); }
 
 template <int DT>
 __device__ __forceinline__ float logit_at(const uint8_t* row, uint32_t c) {
@@ -27,88 +56,278 @@ __device__ __forceinline__ float logit_at(const uint8_t* row, uint32_t c) {
     else return (float)reinterpret_cast<const _Float16*>(row)[slot];
 }
 
-// One workgroup per row: a pass for the maximum, one for the sums, one for each top token.
+// element i of a lane's 16 bytes
 template <int DT>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobsArgs a) {
+__device__ __forceinline__ float logit_of(u32x4 w, int i) {
+    if constexpr (DT == IOMX_DT_F32) return as_f32(w[i]);
+    else if constexpr (DT == IOMX_DT_BF16) return (i & 1) ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]);
+    else { const f32x2 p = f16_pair(w[i >> 1]); return (i & 1) ? p.y : p.x; }
+}
+
+// GT: tiles of a group, which a wave loads at once
+template <int DT, int GT, bool ENTROPY>
+__global__ __launch_bounds__(256) void token_logprobs_scan_kernel(const LogprobsArgs a) {
+    constexpr int kSize = DT == IOMX_DT_F32 ? 4 : 2, kElems = 16 / kSize, kPerRow = kTile / kElems;
+    constexpr int kLoads = GT * 256 * kSize / 1024;
     constexpr float inf = __builtin_inff();
-    __shared__ float shared_a[4], shared_b[4];
-    __shared__ uint32_t shared_i[4];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    const uint32_t plane_index = divided(blockIdx.x, a.R, a.div_rows);
-    const uint32_t r = blockIdx.x - plane_index * a.R;
+    __shared__ float joined[3][4][kTile];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t band = divided(blockIdx.x, a.splits, a.div_splits), split = blockIdx.x - band * a.splits;
+    const uint32_t plane_index = divided(band, a.bands, a.div_bands), tile_row = band - plane_index * a.bands;
+    uint64_t plane[6];
+    walk_planes(a.walk, plane_index, plane);
+    const uint8_t* base = a.logits + (plane[0] * a.logits_plane + (uint64_t)tile_row * a.tile_cols * kTileSlots) * kSize;
+    const uint32_t row = lane / kPerRow % kTile, part = lane % kPerRow;
+    const bool there = tile_row * kTile + row < a.R;
+    const uint32_t lane_tile = lane / (kPerRow * kTile);      // of a load: 1 in the upper half of a wave, 16-bit leaves
+
+    float most = -inf, sum = 0.0f, weighted = 0.0f;           // M (-inf before the first finite logit)
+    const uint32_t c_end = (split + 1) * a.cells_per_split < a.cells ? (split + 1) * a.cells_per_split : a.cells;
+    auto load = [&](uint32_t g, u32x4 (&w)[kLoads]) {
+        const uint8_t* at = base + (uint64_t)g * (GT * kTileSlots * kSize) + lane * 16;
+        if ((g + 1) * GT <= a.tile_cols && there) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) w[i] = *reinterpret_cast<const u32x4*>(at + i * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                w[i] = u32x4{0, 0, 0, 0};
+                if (there && g * GT + i * (GT / kLoads ? GT / kLoads : 1) + lane_tile < a.tile_cols)
+                    w[i] = *reinterpret_cast<const u32x4*>(at + i * 1024);
+            }
+        }
+    };
+    u32x4 next[kLoads];
+    const uint32_t c_begin = split * a.cells_per_split + wave;
+    if (c_begin < c_end) load(c_begin * a.cell_groups, next);
+    for (uint32_t c = c_begin; c < c_end; c += 4) {
+        float cell = -inf;
+        for (uint32_t k = 0; k < a.cell_groups; ++k) {
+            const uint32_t g = c * a.cell_groups + k;
+            if (g * GT >= a.tile_cols) break;
+            u32x4 w[kLoads];
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) w[i] = next[i];
+            const bool more = k + 1 < a.cell_groups && (g + 1) * GT < a.tile_cols;
+            const uint32_t g_next = more ? g + 1 : (c + 4) * a.cell_groups;
+            if (more || c + 4 < c_end) load(g_next, next);
+            // columns from here on are none of the row's
+            const uint32_t columns = a.V - g * (GT * kTile);
+            const bool whole = columns >= (uint32_t)GT * kTile && there;
+            auto logit = [&](int i, int j) {
+                const float x = logit_of<DT>(w[i], j);
+                if (whole) return x;
+                const uint32_t column = (i * (GT / kLoads ? GT / kLoads : 1) + lane_tile) * kTile + part * kElems + j;
+                return there && column < columns ? x : -inf;
+            };
+            auto group = [&](auto x_of) {
+                float top = -inf;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+                    for (int j = 0; j < kElems; j += 2) top = fmaxf(fmaxf(top, x_of(i, j)), x_of(i, j + 1));
+                cell = fmaxf(cell, top);
+                const float m2 = fmaxf(most, top);
+                const float now = m2 == -inf ? 0.0f : m2;
+                // the sums move from the old maximum to the new one: sum d e^d over d + (old - new)
+                const float by = most == -inf ? 0.0f : most - now, factor = exponential(by);
+                if (ENTROPY) weighted = (weighted + at_least(by) * sum) * factor;
+                sum *= factor;
+                most = m2;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+                    for (int j = 0; j < kElems; ++j) {
+                        const float d = x_of(i, j) - now;
+                        const float e = exponential(d);
+                        sum += e;
+                        if (ENTROPY) weighted = __builtin_fmaf(at_least(d), e, weighted);
+                    }
+            };
+            if (columns >= (uint32_t)GT * kTile) group([&](int i, int j) { return logit_of<DT>(w[i], j); });
+            else group(logit);
+        }
+        if (a.cell_max) {
+            // the lanes of a row: neighbours, and the other half of the wave where a load has two tiles
+            cell = fmaxf(cell, __shfl_xor(cell, 1));
+            if constexpr (kPerRow == 4) cell = fmaxf(cell, __shfl_xor(cell, 2));
+            else cell = fmaxf(cell, __shfl_xor(cell, 32));
+            if (there && part == 0 && lane_tile == 0) a.cell_max[((uint64_t)band * a.cells + c) * kTile + row] = cell;
+        }
+    }
+    auto join = [&](float m2, float s2, float w2) {
+        const float m3 = fmaxf(most, m2), now = m3 == -inf ? 0.0f : m3;
+        const float by1 = most == -inf ? 0.0f : most - now, by2 = m2 == -inf ? 0.0f : m2 - now;
+        const float f1 = exponential(by1), f2 = exponential(by2);
+        if (ENTROPY) weighted = (weighted + at_least(by1) * sum) * f1 + (w2 + at_least(by2) * s2) * f2;
+        sum = sum * f1 + s2 * f2;
+        most = m3;
+    };
+    auto join_lanes = [&](int off) {
+        const float m2 = __shfl_xor(most, off), s2 = __shfl_xor(sum, off), w2 = __shfl_xor(weighted, off);
+        join(m2, s2, w2);
+    };
+    join_lanes(1);
+    join_lanes(kPerRow == 4 ? 2 : 32);
+    if (part == 0 && lane_tile == 0) {
+        joined[0][wave][row] = most;
+        joined[1][wave][row] = sum;
+        joined[2][wave][row] = weighted;
+    }
+    __syncthreads();
+    if (threadIdx.x >= kTile) return;
+    most = -inf; sum = 0.0f; weighted = 0.0f;
+    for (int w = 0; w < 4; ++w) join(joined[0][w][lane], joined[1][w][lane], joined[2][w][lane]);
+    float* to = a.stats + (((uint64_t)band * a.splits + split) * kTile + lane) * 4;
+    to[0] = most;
+    to[1] = sum;
+    to[2] = weighted;
+}
+
+// Order of the top: the larger value, of equal ones the lower id, as one number (+0 and -0 are equal).
+__device__ __forceinline__ uint64_t top_key(float x, uint32_t id) {
+    const uint32_t b = as_u32(x == 0.0f ? 0.0f : x);
+    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - id);
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const LogprobsArgs a) {
+    constexpr int kSize = DT == IOMX_DT_F32 ? 4 : 2;
+    constexpr float inf = __builtin_inff();
+    __shared__ uint64_t found[4][kMostCandidates];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t index = blockIdx.x * 4 + wave;          // of the row
+    if (index >= a.rows) return;
+    const uint32_t plane_index = divided(index, a.R, a.div_rows), r = index - plane_index * a.R;
+    const uint32_t band = plane_index * a.bands + (r >> 4);
     uint64_t plane[6];
     walk_planes(a.walk, plane_index, plane);
     const uint8_t* row = a.logits + (plane[0] * a.logits_plane + (uint64_t)(r >> 4) * a.tile_cols * kTileSlots
-                                     + (r & 15u) * kTile) * (DT == IOMX_DT_F32 ? 4 : 2);
-    // the maximum; a NaN or +inf shows as bad
-    float m = -inf;
-    bool bad = false;
-    for (uint32_t c = tid; c < a.V; c += 256) {
-        const float x = logit_at<DT>(row, c);
-        bad = bad || !(x < inf);
-        m = x > m ? x : m;
+                                     + (r & 15u) * kTile) * kSize;
+    // the splits' sums, one per lane (there are 64 at the most)
+    float most = -inf, sum = 0.0f, weighted = 0.0f;
+    if (lane < a.splits) {
+        const float* from = a.stats + (((uint64_t)band * a.splits + lane) * kTile + (r & 15u)) * 4;
+        most = from[0]; sum = from[1]; weighted = from[2];
     }
+    float m = most;
+#pragma unroll
     for (int off = 1; off < 64; off *= 2) m = fmaxf(m, __shfl_xor(m, off));
-    if (lane == 0) shared_a[wave] = m;
-    bad = __syncthreads_or(bad) != 0;
-    m = fmaxf(fmaxf(shared_a[0], shared_a[1]), fmaxf(shared_a[2], shared_a[3]));
-    bad = bad || m == -inf;
-    __syncthreads();
-    float sum = 0.0f, weighted = 0.0f;     // sum e^(x - m), sum (x - m) e^(x - m)
-    for (uint32_t c = tid; c < a.V; c += 256) {
-        const float x = logit_at<DT>(row, c);
-        if (x == -inf) continue;
-        const float e = expf(x - m);
-        sum += e;
-        weighted += (x - m) * e;
-    }
+    const float now = m == -inf ? 0.0f : m, by = most == -inf ? 0.0f : most - now, factor = exponential(by);
+    weighted = (weighted + at_least(by) * sum) * factor;
+    sum *= factor;
+#pragma unroll
     for (int off = 1; off < 64; off *= 2) {
         sum += __shfl_xor(sum, off);
         weighted += __shfl_xor(weighted, off);
     }
-    if (lane == 0) { shared_a[wave] = sum; shared_b[wave] = weighted; }
-    __syncthreads();
-    sum = shared_a[0] + shared_a[1] + shared_a[2] + shared_a[3];
-    weighted = shared_b[0] + shared_b[1] + shared_b[2] + shared_b[3];
-    __syncthreads();
-    const float log_sum = logf(sum), nan = as_f32(kQuietNanF32);
+    // a NaN or +inf left the sum a NaN
+    const bool bad = !(sum > 0.0f);
+    const float nan = as_f32(kQuietNanF32);
+    const double log_sum = log((double)sum), whole = (double)now + log_sum;
     const uint64_t row_at = (uint64_t)(r >> 4), in_row = (r & 15u) * kTile;
-    for (uint32_t g = tid; a.tokens && g < a.G; g += 256) {
+    for (uint32_t g = lane; a.tokens && g < a.G; g += 64) {
         const uint64_t at = (row_at * a.given_tile_cols + (g >> 4)) * kTileSlots + in_row + (g & 15u);
         const uint32_t id = (uint32_t)a.tokens[plane[1] * a.given_plane + at];
-        a.logprobs[plane[2] * a.given_plane + at] = id >= a.V ? -inf : bad ? nan : logit_at<DT>(row, id) - m - log_sum;
+        a.logprobs[plane[2] * a.given_plane + at] = id >= a.V ? -inf : bad ? nan : (float)((double)logit_at<DT>(row, id) - whole);
     }
-    if (a.entropy && tid == 0)
-        a.entropy[plane[3] * a.entropy_plane + row_at * kTileSlots + in_row] = bad ? nan : log_sum - weighted / sum;
+    if (a.entropy && lane == 0)
+        a.entropy[plane[3] * a.entropy_plane + row_at * kTileSlots + in_row] = bad ? nan : (float)(log_sum - (double)weighted / sum);
     if (!a.top_ids) return;
-    float last = inf;
-    uint32_t last_id = 0;
-    for (uint32_t k = 0; k < a.K; ++k) {
-        float best = -inf;
-        uint32_t best_id = 0xFFFFFFFFu;
-        for (uint32_t c = tid; c < a.V; c += 256) {
-            const float x = logit_at<DT>(row, c);
-            const bool after = k == 0 || x < last || (x == last && c > last_id);
-            if (after && (x > best || best_id == 0xFFFFFFFFu)) { best = x; best_id = c; }
+    auto put = [&](uint32_t place, uint64_t key) {
+        const uint64_t at = (row_at * a.top_tile_cols + (place >> 4)) * kTileSlots + in_row + (place & 15u);
+        const uint32_t id = 0xFFFFFFFFu - (uint32_t)key;
+        a.top_ids[plane[4] * a.top_plane + at] = bad ? -1 : (int32_t)id;
+        a.top_logprobs[plane[5] * a.top_plane + at] = bad ? nan : (float)((double)logit_at<DT>(row, id) - whole);
+    };
+    if (bad) {
+        if (lane < a.K) put(lane, 0xFFFFFFFFull);           // id 0, not shown
+        return;
+    }
+    // the K-th largest cell maximum: the largest are taken out, all equal ones at once, until there
+    // are K of them
+    const float* maxima = a.cell_max + (uint64_t)band * a.cells * kTile + (r & 15u);
+    float cells[kMostCells / 64], least = -inf;
+#pragma unroll
+    for (uint32_t i = 0; i < kMostCells / 64; ++i) {
+        const uint32_t c = i * 64 + lane;
+        cells[i] = c < a.cells ? maxima[(uint64_t)c * kTile] : -inf;
+    }
+    uint32_t taken = 0;
+    if (a.cells >= a.K) {
+        float below = inf;                                   // what is taken is not below this
+        while (taken < a.K) {
+            float top = -inf;
+#pragma unroll
+            for (uint32_t i = 0; i < kMostCells / 64; ++i)
+                if (i * 64 < a.cells) top = fmaxf(top, cells[i] < below ? cells[i] : -inf);
+#pragma unroll
+            for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
+            least = below = top;
+            if (top == -inf) break;
+#pragma unroll
+            for (uint32_t i = 0; i < kMostCells / 64; ++i)
+                if (i * 64 < a.cells) taken += __popcll(__ballot(cells[i] == top));
         }
-        auto better = [&](float x, uint32_t id) {
-            if (x > best || (x == best && id < best_id)) { best = x; best_id = id; }
-        };
+    }
+    // the logits that reach it
+    uint32_t count = 0;
+    if (least > -inf) {
+        const uint32_t per_cell = a.cell_groups * a.group_tiles;   // tiles
+#pragma unroll
+        for (uint32_t i = 0; i < kMostCells / 64; ++i) {
+            if (i * 64 >= a.cells) break;
+            uint64_t reach = __ballot(cells[i] >= least);
+            while (reach && count <= kMostCandidates) {
+                const uint32_t c = i * 64 + __ffsll((unsigned long long)reach) - 1;
+                reach &= reach - 1;
+                // four columns of a tile for each lane, sixteen tiles at a time
+                for (uint32_t t = 0; t < per_cell && count <= kMostCandidates; t += 16) {
+                    const uint32_t tile = t + (lane >> 2);
+                    const uint32_t column = (c * per_cell + tile) * kTile + (lane & 3u) * 4;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const bool in = tile < per_cell && column + j < a.V;
+                        const float x = in ? logit_at<DT>(row, column + j) : -inf;
+                        const uint64_t chosen = __ballot(x >= least);
+                        const uint32_t place = count + __popcll(chosen & ((1ull << lane) - 1));
+                        if (x >= least && place < kMostCandidates) found[wave][place] = top_key(x, column + j);
+                        count += __popcll(chosen);
+                    }
+                }
+            }
+        }
+    }
+    if (count >= a.K && count <= kMostCandidates) {
+        // a wave's LDS operations are in order; its own writes are seen
+        __builtin_amdgcn_wave_barrier();
+        const uint64_t one = lane < count ? found[wave][lane] : 0, two = lane + 64 < count ? found[wave][lane + 64] : 0;
+        uint32_t before_one = 0, before_two = 0;
+        for (uint32_t i = 0; i < count; ++i) {
+            const uint64_t key = found[wave][i];
+            before_one += key > one;
+            before_two += key > two;
+        }
+        if (lane < count && before_one < a.K) put(before_one, one);
+        if (lane + 64 < count && before_two < a.K) put(before_two, two);
+        return;
+    }
+    // Too few cells to bound the K-th logit, or too many logits at the bound (rows of equal ones): a
+    // pass over the row for each place.
+    uint64_t last = ~0ull;
+    for (uint32_t place = 0; place < a.K; ++place) {
+        uint64_t best = 0;
+        for (uint32_t c = lane; c < a.V; c += 64) {
+            const uint64_t key = top_key(logit_at<DT>(row, c), c);
+            best = key < last && key > best ? key : best;
+        }
+#pragma unroll
         for (int off = 1; off < 64; off *= 2) {
-            const float x = __shfl_xor(best, off);
-            better(x, __shfl_xor(best_id, off));
+            const uint64_t other = __shfl_xor((unsigned long long)best, off);
+            best = other > best ? other : best;
         }
-        if (lane == 0) { shared_a[wave] = best; shared_i[wave] = best_id; }
-        __syncthreads();
-        for (uint32_t w = 0; w < 4; ++w) better(shared_a[w], shared_i[w]);
-        __syncthreads();
         last = best;
-        last_id = best_id;
-        if (tid == 0) {
-            const uint64_t at = (row_at * a.top_tile_cols + (k >> 4)) * kTileSlots + in_row + (k & 15u);
-            a.top_ids[plane[4] * a.top_plane + at] = bad ? -1 : (int32_t)best_id;
-            a.top_logprobs[plane[5] * a.top_plane + at] = bad ? nan : best - m - log_sum;
-        }
+        if (lane == 0) put(place, best);
     }
 }
 
@@ -158,6 +377,9 @@ int logprobs_request(int dtype, const iomx_view* logits, const iomx_view* tokens
     a->V = (uint32_t)m.cols;
     a->tile_cols = (uint32_t)m.tile_cols;
     a->div_rows = make_fast_div(a->R);
+    a->rows = (uint32_t)rows;
+    a->bands = (uint32_t)m.tile_rows;
+    a->div_bands = make_fast_div(a->bands);
     if (tokens) {
         const Matrix g = matrix_of(*tokens);
         a->tokens = static_cast<const int32_t*>(tokens->base);
@@ -181,6 +403,39 @@ int logprobs_request(int dtype, const iomx_view* logits, const iomx_view* tokens
     return IOMX_OK;
 }
 
+// The scan's layout, and the floats of workspace it takes.
+int logprobs_layout(LogprobsArgs* a, uint64_t* stats_floats, uint64_t* cell_floats) {
+    // groups of 64 columns for small vocabularies, so that even a row of few thousand logits has a
+    // cell for each of the K most likely; cells of several groups where there would be too many
+    a->group_tiles = a->V < 16384 ? 4 : 16;
+    const uint32_t groups = (a->tile_cols + a->group_tiles - 1) / a->group_tiles;
+    a->cell_groups = (groups + kMostCells - 1) / kMostCells;
+    a->cells = (groups + a->cell_groups - 1) / a->cell_groups;
+    // six workgroups for each CU in all, a cell for each wave at the least
+    const uint64_t bands = a->walk.planes * a->bands;
+    uint64_t splits = bands >= 1536 ? 1 : (1536 + bands - 1) / bands;
+    if (splits > (a->cells + 3) / 4) splits = (a->cells + 3) / 4;
+    if (splits > 64) splits = 64;
+    a->cells_per_split = (uint32_t)((a->cells + splits - 1) / splits);
+    a->splits = (a->cells + a->cells_per_split - 1) / a->cells_per_split;
+    a->div_splits = make_fast_div(a->splits);
+    if (bands * a->splits > 0x7FFFFFF0ull) return IOMX_ERR_OVERFLOW;
+    *stats_floats = bands * a->splits * kTile * 4;
+    *cell_floats = a->top_ids ? bands * a->cells * kTile : 0;
+    return IOMX_OK;
+}
+
+template <int DT>
+void launch_logprobs(const LogprobsArgs& a, hipStream_t st) {
+    const dim3 grid((uint32_t)(a.walk.planes * a.bands * a.splits));
+    if (a.group_tiles == 4 && a.entropy) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 4, true>), grid, dim3(256), 0, st, a);
+    else if (a.group_tiles == 4) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 4, false>), grid, dim3(256), 0, st, a);
+    else if (a.entropy) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 16, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 16, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL(token_logprobs_finish_kernel<DT>, dim3((a.rows + 3) / 4), dim3(256), 0, st, a);
+    record_launch("token_logprobs", grid.x, 256, (uint64_t)a.rows * a.V);
+}
+
 }  // namespace
 
 }  // namespace iomx
@@ -194,8 +449,10 @@ extern "C" int iomx_token_logprobs_workspace(int dtype, const iomx_view* logits,
     if (!bytes || !alignment) return IOMX_ERR_INVALID;
     LogprobsArgs a = {};
     IOMX_TRY(logprobs_request(dtype, logits, tokens, logprobs, entropy, top_ids, top_logprobs, &a));
-    *bytes = 0;
-    *alignment = 1;
+    uint64_t stats, cells;
+    IOMX_TRY(logprobs_layout(&a, &stats, &cells));
+    *bytes = (stats + cells) * 4;
+    *alignment = 256;
     return IOMX_OK;
 }
 
@@ -203,16 +460,18 @@ extern "C" int iomx_launch_token_logprobs(int dtype, const iomx_view* logits, co
                                           const iomx_view* logprobs, const iomx_view* entropy,
                                           const iomx_view* top_ids, const iomx_view* top_logprobs,
                                           void* workspace, uint64_t workspace_bytes, iomx_stream_t stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     LogprobsArgs a = {};
     IOMX_TRY(logprobs_request(dtype, logits, tokens, logprobs, entropy, top_ids, top_logprobs, &a));
-    const dim3 grid((uint32_t)(a.walk.planes * a.R));
+    uint64_t stats, cells;
+    IOMX_TRY(logprobs_layout(&a, &stats, &cells));
+    if (!workspace || workspace_bytes < (stats + cells) * 4 || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+        return IOMX_ERR_INVALID;
+    a.stats = static_cast<float*>(workspace);
+    a.cell_max = cells ? a.stats + stats : nullptr;
     const hipStream_t st = native(stream);
-    if (dtype == IOMX_DT_BF16) hipLaunchKernelGGL(token_logprobs_kernel<IOMX_DT_BF16>, grid, dim3(256), 0, st, a);
-    else if (dtype == IOMX_DT_F16) hipLaunchKernelGGL(token_logprobs_kernel<IOMX_DT_F16>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(token_logprobs_kernel<IOMX_DT_F32>, grid, dim3(256), 0, st, a);
-    record_launch("token_logprobs", grid.x, 256, (uint64_t)grid.x * a.V);
+    if (dtype == IOMX_DT_BF16) launch_logprobs<IOMX_DT_BF16>(a, st);
+    else if (dtype == IOMX_DT_F16) launch_logprobs<IOMX_DT_F16>(a, st);
+    else launch_logprobs<IOMX_DT_F32>(a, st);
     IOMX_HIP(hipGetLastError());
     return IOMX_OK;
 }

@@ -283,7 +283,10 @@ struct PackedTiles {
 // launch counts on, and looks up its own piece in the running count.  A launch has a workgroup for
 // every piece of that size and one more for every row block (pieces are rounded up).
 constexpr uint32_t kPackedGroups = 512, kPackedGroupsLog2 = 9;   // workgroups to share out to
-constexpr uint32_t kPackedLeastBlocks = 4;                        // of tokens, in a piece
+// Tokens of a piece at the least.  A piece costs a second launch and its sums' way through memory:
+// sixteen sequences of up to 509 cached tokens and one row each (4 KV heads of 64) take 9.3 us on 64
+// workgroups and 12.3 us in pieces of 128.
+constexpr uint32_t kPackedLeastTokens = 512;
 
 struct PackedShare {
     uint32_t s, row_block, piece, pieces, size;   // size: token blocks of a piece
@@ -315,7 +318,8 @@ __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uin
     for (int off = 1; off < 64; off *= 2) total += __shfl_xor((unsigned long long)total, off);
     PackedShare p = {};
     const uint64_t even = (total * a.Hkv + kPackedGroups - 1) >> kPackedGroupsLog2;
-    p.size = even > kPackedLeastBlocks ? (uint32_t)even : kPackedLeastBlocks;
+    constexpr uint32_t least = kPackedLeastTokens / (16 * NT);
+    p.size = even > least ? (uint32_t)even : least;
     p.s = ~0u;
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
@@ -991,8 +995,7 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
     // Shared out where there are fewer row blocks than two per CU and a sequence may have tokens for
     // more than one piece.
     const uint64_t capacity = (uint64_t)a.table.cols * a.page_rows + a.max_rows;
-    const uint64_t least = kPackedLeastBlocks * (p->row_waves == 4 ? 64 : 32);
-    if (p->groups < kPackedGroups && capacity > 2 * least) {
+    if (p->groups < kPackedGroups && capacity > 2 * kPackedLeastTokens) {
         p->shared_out = true;
         p->groups += (kPackedGroups + a.Hkv - 1) / a.Hkv * (uint64_t)a.Hkv;
         p->stats_floats = (p->groups * p->block_rows * 2 + 63) / 64 * 64;
