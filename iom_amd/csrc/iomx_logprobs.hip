@@ -1,7 +1,11 @@
 // Log probabilities of given tokens, entropy and the most likely tokens of vocabulary rows.
+#include <type_traits>
+
 #include "iomx_packed.hpp"
 
 namespace iomx {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kMaxTop = 32;
 
@@ -35,12 +39,13 @@ struct LogprobsArgs {
 // exponential per logit keep the vector units at about two thirds of what the memory leaves them.
 //
 // token_logprobs_finish, one wave per row, joins the sums and picks the most likely tokens without
-// another pass: the K-th largest cell maximum bounds the K-th largest logit from below, so only the
-// cells that reach it are read again, and in them the logits that reach it are few; each counts
-// those before it (larger, or equal with a lower id), which is its place.
+// another pass: a value that K cells' maxima reach is reached by K logits, so only the cells that
+// reach it are read again, and in them the logits that reach it are few; each counts those before it
+// (larger, or equal with a lower id), which is its place.
 // ---------------------------------------------------------------------------
 
 constexpr uint32_t kMostCells = 1024;         // of a row: sixteen per lane
+constexpr uint32_t kMostChosen = 256;         // cells that are read again
 constexpr uint32_t kMostCandidates = 128;     // of a row: two per lane
 
 // d as a factor of e^d: from -200 on down e^d is 0 in F32, and its product with d is, too
@@ -189,14 +194,37 @@ __device__ __forceinline__ uint64_t top_key(float x, uint32_t id) {
     const uint32_t b = as_u32(x == 0.0f ? 0.0f : x);
     return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - id);
 }
+__device__ __forceinline__ uint32_t key_id(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t b = (uint32_t)(key >> 32);
+    return as_f32(b & 0x80000000u ? b & 0x7FFFFFFFu : ~b);
+}
+
+// Reductions over a wave by moves within the register file (a shuffle goes through LDS): rows of 16
+// lanes by four rotations, then the rows' results by two broadcasts.
+__device__ __forceinline__ float wave_max(float x) {
+    auto moved = [](float v, auto control) __attribute__((always_inline)) {
+        constexpr int kControl = decltype(control)::value;
+        return as_f32(__builtin_amdgcn_update_dpp(as_u32(v), as_u32(v), kControl, 0xF, 0xF, false));
+    };
+    x = fmaxf(x, moved(x, std::integral_constant<int, 0x121>{}));   // row_ror:1, 2, 4, 8
+    x = fmaxf(x, moved(x, std::integral_constant<int, 0x122>{}));
+    x = fmaxf(x, moved(x, std::integral_constant<int, 0x124>{}));
+    x = fmaxf(x, moved(x, std::integral_constant<int, 0x128>{}));
+    const float a = as_f32(__builtin_amdgcn_readlane(as_u32(x), 0)), b = as_f32(__builtin_amdgcn_readlane(as_u32(x), 16));
+    const float c = as_f32(__builtin_amdgcn_readlane(as_u32(x), 32)), d = as_f32(__builtin_amdgcn_readlane(as_u32(x), 48));
+    return fmaxf(fmaxf(a, b), fmaxf(c, d));
+}
 
 template <int DT>
 __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const LogprobsArgs a) {
     constexpr int kSize = DT == IOMX_DT_F32 ? 4 : 2;
     constexpr float inf = __builtin_inff();
+    constexpr uint32_t kSlots = kMostCells / 64;
     __shared__ uint64_t found[4][kMostCandidates];
+    __shared__ uint16_t chosen[4][kMostChosen];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t index = blockIdx.x * 4 + wave;          // of the row
+    const uint32_t index = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);          // of the row
     if (index >= a.rows) return;
     const uint32_t plane_index = divided(index, a.R, a.div_rows), r = index - plane_index * a.R;
     const uint32_t band = plane_index * a.bands + (r >> 4);
@@ -204,15 +232,23 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
     walk_planes(a.walk, plane_index, plane);
     const uint8_t* row = a.logits + (plane[0] * a.logits_plane + (uint64_t)(r >> 4) * a.tile_cols * kTileSlots
                                      + (r & 15u) * kTile) * kSize;
-    // the splits' sums, one per lane (there are 64 at the most)
+    // everything that the workspace holds of the row, in one go: the cells' maxima ...
+    float cells[kSlots];
+    if (a.top_ids) {
+        const float* maxima = a.cell_max + (uint64_t)band * a.cells * kTile + (r & 15u);
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) {
+            const uint32_t c = i * 64 + lane;
+            cells[i] = c < a.cells ? maxima[(uint64_t)c * kTile] : -inf;
+        }
+    }
+    // ... and the splits' sums, one per lane (there are 64 at the most)
     float most = -inf, sum = 0.0f, weighted = 0.0f;
     if (lane < a.splits) {
-        const float* from = a.stats + (((uint64_t)band * a.splits + lane) * kTile + (r & 15u)) * 4;
+        const f32x4_t from = *reinterpret_cast<const f32x4_t*>(a.stats + (((uint64_t)band * a.splits + lane) * kTile + (r & 15u)) * 4);
         most = from[0]; sum = from[1]; weighted = from[2];
     }
-    float m = most;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) m = fmaxf(m, __shfl_xor(m, off));
+    const float m = wave_max(most);
     const float now = m == -inf ? 0.0f : m, by = most == -inf ? 0.0f : most - now, factor = exponential(by);
     weighted = (weighted + at_least(by) * sum) * factor;
     sum *= factor;
@@ -234,82 +270,115 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
     if (a.entropy && lane == 0)
         a.entropy[plane[3] * a.entropy_plane + row_at * kTileSlots + in_row] = bad ? nan : (float)(log_sum - (double)weighted / sum);
     if (!a.top_ids) return;
-    auto put = [&](uint32_t place, uint64_t key) {
+    auto put = [&](uint32_t place, uint32_t id, float logit) {
         const uint64_t at = (row_at * a.top_tile_cols + (place >> 4)) * kTileSlots + in_row + (place & 15u);
-        const uint32_t id = 0xFFFFFFFFu - (uint32_t)key;
         a.top_ids[plane[4] * a.top_plane + at] = bad ? -1 : (int32_t)id;
-        a.top_logprobs[plane[5] * a.top_plane + at] = bad ? nan : (float)((double)logit_at<DT>(row, id) - whole);
+        a.top_logprobs[plane[5] * a.top_plane + at] = bad ? nan : (float)((double)logit - whole);
     };
     if (bad) {
-        if (lane < a.K) put(lane, 0xFFFFFFFFull);           // id 0, not shown
+        if (lane < a.K) put(lane, 0, 0.0f);
         return;
     }
-    // the K-th largest cell maximum: the largest are taken out, all equal ones at once, until there
-    // are K of them
-    const float* maxima = a.cell_max + (uint64_t)band * a.cells * kTile + (r & 15u);
-    float cells[kMostCells / 64], least = -inf;
+    // A bound that at least K cells' maxima reach, so that at least K logits do, and not many more: from
+    // the row's maximum downwards in steps that double, then halving the last step.
+    auto reaching = [&](float bound) __attribute__((always_inline)) -> uint32_t {
+        uint32_t n = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kMostCells / 64; ++i) {
-        const uint32_t c = i * 64 + lane;
-        cells[i] = c < a.cells ? maxima[(uint64_t)c * kTile] : -inf;
-    }
-    uint32_t taken = 0;
+        for (uint32_t i = 0; i < kSlots; ++i)
+            if (i * 64 < a.cells) n += __popcll(__ballot(cells[i] >= bound));
+        return n;
+    };
+    float bound = -inf;
+    uint32_t reached = 0;
     if (a.cells >= a.K) {
-        float below = inf;                                   // what is taken is not below this
-        while (taken < a.K) {
-            float top = -inf;
+        float top = cells[0];
 #pragma unroll
-            for (uint32_t i = 0; i < kMostCells / 64; ++i)
-                if (i * 64 < a.cells) top = fmaxf(top, cells[i] < below ? cells[i] : -inf);
-#pragma unroll
-            for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
-            least = below = top;
-            if (top == -inf) break;
-#pragma unroll
-            for (uint32_t i = 0; i < kMostCells / 64; ++i)
-                if (i * 64 < a.cells) taken += __popcll(__ballot(cells[i] == top));
+        for (uint32_t i = 1; i < kSlots; ++i) top = fmaxf(top, cells[i]);
+        top = wave_max(top);
+        float over = top, step = fmaxf(1.0f, fabsf(top) * 0.0078125f);   // `over`: fewer than K reach it, or it is the top
+        for (;;) {
+            bound = top - step;
+            reached = reaching(bound);
+            if (reached >= a.K || bound == -inf) break;
+            over = bound;
+            step *= 2.0f;
+        }
+        for (int halvings = 0; halvings < 12 && reached > a.K + a.K / 2; ++halvings) {
+            const float middle = bound + (over - bound) * 0.5f;
+            const uint32_t n = reaching(middle);
+            if (n >= a.K) { bound = middle; reached = n; }
+            else over = middle;
         }
     }
     // the logits that reach it
     uint32_t count = 0;
-    if (least > -inf) {
-        const uint32_t per_cell = a.cell_groups * a.group_tiles;   // tiles
+    if (bound > -inf && reached <= kMostChosen) {
+        uint32_t listed = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kMostCells / 64; ++i) {
+        for (uint32_t i = 0; i < kSlots; ++i) {
             if (i * 64 >= a.cells) break;
-            uint64_t reach = __ballot(cells[i] >= least);
-            while (reach && count <= kMostCandidates) {
-                const uint32_t c = i * 64 + __ffsll((unsigned long long)reach) - 1;
-                reach &= reach - 1;
-                // four columns of a tile for each lane, sixteen tiles at a time
-                for (uint32_t t = 0; t < per_cell && count <= kMostCandidates; t += 16) {
-                    const uint32_t tile = t + (lane >> 2);
-                    const uint32_t column = (c * per_cell + tile) * kTile + (lane & 3u) * 4;
+            const uint64_t there = __ballot(cells[i] >= bound);
+            if (cells[i] >= bound) chosen[wave][listed + __popcll(there & ((1ull << lane) - 1))] = (uint16_t)(i * 64 + lane);
+            listed += __popcll(there);
+        }
+        __builtin_amdgcn_wave_barrier();       // a wave's LDS operations are in order
+        // A lane takes four columns of a tile; a wave, sixteen tiles: a part of one cell, or four cells.
+        // The loads of eight such pieces are on their way together.
+        constexpr uint32_t kAhead = 8;
+        const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 16
+        const uint32_t parts = per_cell < 16 ? 1 : per_cell / 16, together = per_cell < 16 ? 4 : 1;
+        const uint32_t pieces = (listed + together - 1) / together * parts;
+        for (uint32_t p0 = 0; p0 < pieces && count <= kMostCandidates; p0 += kAhead) {
+            float x[kAhead][4];
+            uint32_t first[kAhead];
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        const bool in = tile < per_cell && column + j < a.V;
-                        const float x = in ? logit_at<DT>(row, column + j) : -inf;
-                        const uint64_t chosen = __ballot(x >= least);
-                        const uint32_t place = count + __popcll(chosen & ((1ull << lane) - 1));
-                        if (x >= least && place < kMostCandidates) found[wave][place] = top_key(x, column + j);
-                        count += __popcll(chosen);
-                    }
+            for (uint32_t n = 0; n < kAhead; ++n) {
+                const uint32_t p = p0 + n;
+                const uint32_t entry = together == 4 ? p * 4 + (lane >> 4) : p / parts;
+                const uint32_t tile_in_cell = together == 4 ? (lane >> 2) & 3u : p % parts * 16 + (lane >> 2);
+                const uint32_t tile = (entry < listed ? chosen[wave][entry] : 0u) * per_cell + tile_in_cell;
+                first[n] = tile * kTile + (lane & 3u) * 4;
+                const bool in = p < pieces && entry < listed && tile < a.tile_cols;
+                // a tile's padding columns are read with it, and not looked at
+                const uint8_t* at = row + ((uint64_t)(in ? tile : 0u) * kTileSlots + (lane & 3u) * 4) * kSize;
+                if constexpr (DT == IOMX_DT_F32) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[n][j] = as_f32(w[j]);
+                } else {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+                    const u32x4 wide = {w.x, w.y, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[n][j] = logit_of<DT>(wide, j);
                 }
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) x[n][j] = in && first[n] + j < a.V ? x[n][j] : -inf;
             }
+#pragma unroll
+            for (uint32_t n = 0; n < kAhead; ++n)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint64_t there = __ballot(x[n][j] >= bound);
+                    if (!there) continue;
+                    const uint32_t place = count + __popcll(there & ((1ull << lane) - 1));
+                    if (x[n][j] >= bound && place < kMostCandidates) found[wave][place] = top_key(x[n][j], first[n] + j);
+                    count += __popcll(there);
+                }
         }
     }
     if (count >= a.K && count <= kMostCandidates) {
-        // a wave's LDS operations are in order; its own writes are seen
         __builtin_amdgcn_wave_barrier();
         const uint64_t one = lane < count ? found[wave][lane] : 0, two = lane + 64 < count ? found[wave][lane + 64] : 0;
         uint32_t before_one = 0, before_two = 0;
         for (uint32_t i = 0; i < count; ++i) {
-            const uint64_t key = found[wave][i];
+            const uint64_t from = i < 64 ? one : two;
+            const uint64_t key = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(from >> 32), i & 63u) << 32
+                               | (uint32_t)__builtin_amdgcn_readlane((uint32_t)from, i & 63u);
             before_one += key > one;
             before_two += key > two;
         }
-        if (lane < count && before_one < a.K) put(before_one, one);
-        if (lane + 64 < count && before_two < a.K) put(before_two, two);
+        if (lane < count && before_one < a.K) put(before_one, key_id(one), key_value(one));
+        if (lane + 64 < count && before_two < a.K) put(before_two, key_id(two), key_value(two));
         return;
     }
     // Too few cells to bound the K-th logit, or too many logits at the bound (rows of equal ones): a
@@ -327,7 +396,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
             best = other > best ? other : best;
         }
         last = best;
-        if (lane == 0) put(place, best);
+        if (lane == 0) put(place, key_id(best), key_value(best));
     }
 }
 
