@@ -44,7 +44,7 @@ struct LogprobsArgs {
 // (larger, or equal with a lower id), which is its place.
 // ---------------------------------------------------------------------------
 
-constexpr uint32_t kMostCells = 1024;         // of a row: sixteen per lane
+constexpr uint32_t kMostCells = 512;          // of a row: eight per lane
 constexpr uint32_t kMostChosen = 256;         // cells that are read again
 constexpr uint32_t kMostCandidates = 128;     // of a row: two per lane
 
@@ -201,19 +201,26 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 
 // Reductions over a wave by moves within the register file (a shuffle goes through LDS): rows of 16
-// lanes by four rotations, then the rows' results by two broadcasts.
-__device__ __forceinline__ float wave_max(float x) {
-    auto moved = [](float v, auto control) __attribute__((always_inline)) {
-        constexpr int kControl = decltype(control)::value;
-        return as_f32(__builtin_amdgcn_update_dpp(as_u32(v), as_u32(v), kControl, 0xF, 0xF, false));
-    };
-    x = fmaxf(x, moved(x, std::integral_constant<int, 0x121>{}));   // row_ror:1, 2, 4, 8
-    x = fmaxf(x, moved(x, std::integral_constant<int, 0x122>{}));
-    x = fmaxf(x, moved(x, std::integral_constant<int, 0x124>{}));
-    x = fmaxf(x, moved(x, std::integral_constant<int, 0x128>{}));
+// lanes by four rotations, then the rows' results out of scalar registers.
+template <int CONTROL>
+__device__ __forceinline__ float lane_moved(float v) {
+    return as_f32(__builtin_amdgcn_update_dpp(as_u32(v), as_u32(v), CONTROL, 0xF, 0xF, false));
+}
+template <class Op>
+__device__ __forceinline__ float wave_reduce(float x, Op op) {
+    x = op(x, lane_moved<0x121>(x));   // row_ror:1, 2, 4, 8
+    x = op(x, lane_moved<0x122>(x));
+    x = op(x, lane_moved<0x124>(x));
+    x = op(x, lane_moved<0x128>(x));
     const float a = as_f32(__builtin_amdgcn_readlane(as_u32(x), 0)), b = as_f32(__builtin_amdgcn_readlane(as_u32(x), 16));
     const float c = as_f32(__builtin_amdgcn_readlane(as_u32(x), 32)), d = as_f32(__builtin_amdgcn_readlane(as_u32(x), 48));
-    return fmaxf(fmaxf(a, b), fmaxf(c, d));
+    return op(op(a, b), op(c, d));
+}
+__device__ __forceinline__ float wave_max(float x) {
+    return wave_reduce(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    return wave_reduce(x, [](float a, float b) { return a + b; });
 }
 
 template <int DT>
@@ -248,24 +255,31 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
         const f32x4_t from = *reinterpret_cast<const f32x4_t*>(a.stats + (((uint64_t)band * a.splits + lane) * kTile + (r & 15u)) * 4);
         most = from[0]; sum = from[1]; weighted = from[2];
     }
+    // ... and the first 64 given tokens
+    const uint64_t row_at = (uint64_t)(r >> 4), in_row = (r & 15u) * kTile;
+    auto given_at = [&](uint32_t g) { return (row_at * a.given_tile_cols + (g >> 4)) * kTileSlots + in_row + (g & 15u); };
+    uint32_t given = a.V;
+    float given_logit = 0.0f;
+    if (lane < a.G) {
+        given = (uint32_t)a.tokens[plane[1] * a.given_plane + given_at(lane)];
+        if (given < a.V) given_logit = logit_at<DT>(row, given);
+    }
     const float m = wave_max(most);
     const float now = m == -inf ? 0.0f : m, by = most == -inf ? 0.0f : most - now, factor = exponential(by);
     weighted = (weighted + at_least(by) * sum) * factor;
-    sum *= factor;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-        sum += __shfl_xor(sum, off);
-        weighted += __shfl_xor(weighted, off);
-    }
+    sum = wave_sum(sum * factor);
+    weighted = wave_sum(weighted);
     // a NaN or +inf left the sum a NaN
     const bool bad = !(sum > 0.0f);
     const float nan = as_f32(kQuietNanF32);
     const double log_sum = log((double)sum), whole = (double)now + log_sum;
-    const uint64_t row_at = (uint64_t)(r >> 4), in_row = (r & 15u) * kTile;
-    for (uint32_t g = lane; a.tokens && g < a.G; g += 64) {
-        const uint64_t at = (row_at * a.given_tile_cols + (g >> 4)) * kTileSlots + in_row + (g & 15u);
-        const uint32_t id = (uint32_t)a.tokens[plane[1] * a.given_plane + at];
-        a.logprobs[plane[2] * a.given_plane + at] = id >= a.V ? -inf : bad ? nan : (float)((double)logit_at<DT>(row, id) - whole);
+    for (uint32_t g = lane; g < a.G; g += 64) {
+        if (g >= 64) {
+            given = (uint32_t)a.tokens[plane[1] * a.given_plane + given_at(g)];
+            if (given < a.V) given_logit = logit_at<DT>(row, given);
+        }
+        a.logprobs[plane[2] * a.given_plane + given_at(g)] =
+                given >= a.V ? -inf : bad ? nan : (float)((double)given_logit - whole);
     }
     if (a.entropy && lane == 0)
         a.entropy[plane[3] * a.entropy_plane + row_at * kTileSlots + in_row] = bad ? nan : (float)(log_sum - (double)weighted / sum);
@@ -288,13 +302,16 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
             if (i * 64 < a.cells) n += __popcll(__ballot(cells[i] >= bound));
         return n;
     };
-    float bound = -inf;
-    uint32_t reached = 0;
-    if (a.cells >= a.K) {
-        float top = cells[0];
+    auto largest_below = [&](float limit) __attribute__((always_inline)) -> float {
+        float top = -inf;
 #pragma unroll
-        for (uint32_t i = 1; i < kSlots; ++i) top = fmaxf(top, cells[i]);
-        top = wave_max(top);
+        for (uint32_t i = 0; i < kSlots; ++i) top = fmaxf(top, cells[i] < limit ? cells[i] : -inf);
+        return wave_max(top);
+    };
+    float bound = -inf;
+    uint32_t reached = 0, ties = ~0u;              // ties: cells of exactly the bound that are looked at
+    if (a.cells >= a.K) {
+        const float top = largest_below(inf);
         float over = top, step = fmaxf(1.0f, fabsf(top) * 0.0078125f);   // `over`: fewer than K reach it, or it is the top
         for (;;) {
             bound = top - step;
@@ -309,23 +326,42 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
             if (n >= a.K) { bound = middle; reached = n; }
             else over = middle;
         }
-    }
-    // the logits that reach it
-    uint32_t count = 0;
-    if (bound > -inf && reached <= kMostChosen) {
-        uint32_t listed = 0;
+        if (bound > -inf && reached > kMostChosen) {
+            // (rows of equal logits) the K-th largest maximum itself: of the cells that have it, those
+            // with the lowest columns make up the K cells that hold the K most likely tokens
+            uint32_t larger = 0;
+            bound = top;
+            for (;;) {
+                uint32_t equal = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i) {
-            if (i * 64 >= a.cells) break;
-            const uint64_t there = __ballot(cells[i] >= bound);
-            if (cells[i] >= bound) chosen[wave][listed + __popcll(there & ((1ull << lane) - 1))] = (uint16_t)(i * 64 + lane);
-            listed += __popcll(there);
+                for (uint32_t i = 0; i < kSlots; ++i) equal += __popcll(__ballot(cells[i] == bound));
+                if (larger + equal >= a.K) break;
+                larger += equal;
+                bound = largest_below(bound);
+            }
+            ties = a.K - larger;
         }
+    }
+    // fewer than K cells, or than K with a finite maximum: every finite logit
+    if (bound == -inf) bound = -3.4028234663852886e38f;
+    // the logits that reach it
+    uint32_t count = 0, listed = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kSlots; ++i) {
+        if (i * 64 >= a.cells) break;
+        const uint64_t below = (1ull << lane) - 1, equal = __ballot(cells[i] == bound);
+        const bool take = cells[i] > bound || (cells[i] == bound && (uint32_t)__popcll(equal & below) < ties);
+        const uint64_t there = __ballot(take);
+        if (take) chosen[wave][listed + __popcll(there & below)] = (uint16_t)(i * 64 + lane);
+        listed += __popcll(there);
+        if (ties != ~0u) ties -= __popcll(equal) < ties ? __popcll(equal) : ties;
+    }
+    const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 16
+    {
         __builtin_amdgcn_wave_barrier();       // a wave's LDS operations are in order
         // A lane takes four columns of a tile; a wave, sixteen tiles: a part of one cell, or four cells.
         // The loads of eight such pieces are on their way together.
         constexpr uint32_t kAhead = 8;
-        const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 16
         const uint32_t parts = per_cell < 16 ? 1 : per_cell / 16, together = per_cell < 16 ? 4 : 1;
         const uint32_t pieces = (listed + together - 1) / together * parts;
         for (uint32_t p0 = 0; p0 < pieces && count <= kMostCandidates; p0 += kAhead) {
@@ -366,7 +402,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
                 }
         }
     }
-    if (count >= a.K && count <= kMostCandidates) {
+    if (count <= kMostCandidates) {
         __builtin_amdgcn_wave_barrier();
         const uint64_t one = lane < count ? found[wave][lane] : 0, two = lane + 64 < count ? found[wave][lane + 64] : 0;
         uint32_t before_one = 0, before_two = 0;
@@ -379,16 +415,28 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
         }
         if (lane < count && before_one < a.K) put(before_one, key_id(one), key_value(one));
         if (lane + 64 < count && before_two < a.K) put(before_two, key_id(two), key_value(two));
+        // too few finite logits: the first of the others follow
+        uint32_t place = count;
+        for (uint32_t c0 = 0; place < a.K && c0 < a.V; c0 += 64) {
+            const bool masked = c0 + lane < a.V && logit_at<DT>(row, c0 + lane) == -inf;
+            const uint64_t there = __ballot(masked);
+            const uint32_t mine = place + __popcll(there & ((1ull << lane) - 1));
+            if (masked && mine < a.K) put(mine, c0 + lane, -inf);
+            place += __popcll(there);
+        }
         return;
     }
-    // Too few cells to bound the K-th logit, or too many logits at the bound (rows of equal ones): a
-    // pass over the row for each place.
+    // many equal logits at the bound: a pass over the chosen cells for each place
     uint64_t last = ~0ull;
     for (uint32_t place = 0; place < a.K; ++place) {
         uint64_t best = 0;
-        for (uint32_t c = lane; c < a.V; c += 64) {
-            const uint64_t key = top_key(logit_at<DT>(row, c), c);
-            best = key < last && key > best ? key : best;
+        for (uint32_t n = 0; n < listed; ++n) {
+            const uint32_t from = chosen[wave][n] * per_cell * kTile;
+            const uint32_t to = from + per_cell * kTile < a.V ? from + per_cell * kTile : a.V;
+            for (uint32_t c = from + lane; c < to; c += 64) {
+                const uint64_t key = top_key(logit_at<DT>(row, c), c);
+                best = key < last && key > best ? key : best;
+            }
         }
 #pragma unroll
         for (int off = 1; off < 64; off *= 2) {

@@ -232,3 +232,43 @@ def test_the_same_result_every_time_and_recorded():
             assert np.array_equal(got, want[n]), (replay, n)
     graph.close()
     st.close()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [40000, 300001])
+def test_large_vocabularies_of_few_and_of_equal_logits(dtype, V):
+    """Rows with fewer finite logits than places (a grammar that allows a few tokens), rows of equal
+    logits, equal largest logits in many cells, in one cell, and just more of them than places."""
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((12, V)) * 2
+    x[0, :] = -np.inf
+    x[0, rng.permutation(V)[:10]] = rng.standard_normal(10)
+    x[1, :] = -np.inf
+    x[1, rng.permutation(V)[:200]] = rng.standard_normal(200)
+    x[2, :] = 0.25
+    x[3, rng.permutation(V)[:400]] = 20.0
+    x[4, 777:1400] = 20.0
+    x[5, rng.permutation(V)[:33]] = 20.0
+    x[6, rng.permutation(V)[:31]] = 20.0
+    x[7, :] = -np.inf
+    x[7, 5:300] = 1.0                                              # in one or two cells
+    x[8, :] = -np.inf
+    x[8, V - 20:] = 1.0
+    x[9, :] = np.where(np.arange(V) % 3 == 0, -np.inf, -7.0)
+    x[10, V - 1] = 30.0
+    for K in (1, 20, 32):
+        check(dtype, encode(dtype, x), rng.integers(0, V, (12, 2)), K)
+
+
+def test_the_workspace_has_to_be_there():
+    t = {"logits": iomx.DeviceTensor(BF16, (3, 500)), "entropy": iomx.DeviceTensor(F32, (3, 1), fill=0x5A)}
+    views = {n: x.view() for n, x in t.items()}
+    rc, nbytes, align = iomx.token_logprobs_workspace(**views)
+    assert rc == 0 and nbytes > 0 and align == 256
+    small = iomx.Buffer(nbytes - 1)
+    assert iomx.token_logprobs(**views) == iomx.ERR_INVALID
+    assert iomx.token_logprobs(workspace=small, **views) == iomx.ERR_INVALID
+    off = iomx.Buffer(nbytes + 256)
+    assert iomx.token_logprobs(workspace=iomx.Buffer.at(off.ptr.value + 64, nbytes), **views) == iomx.ERR_INVALID
+    iomx.synchronize()
+    assert (t["entropy"].view().to_host() == 0x5A5A5A5A).all()
