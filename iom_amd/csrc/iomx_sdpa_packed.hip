@@ -23,7 +23,8 @@ struct SdpaPackedArgs {
     FastDiv div_group, div_page_rows;
     float scale;                                              // 1 / sqrt(D)
     // the matrix-core kernel
-    uint32_t row_blocks, shared_out;                          // tokens of a row block shared out: see PackedShare
+    uint32_t row_blocks;
+    uint32_t places;                                          // for the pieces of a KV head (PackedShare); 0: not shared out
     uint32_t page_tiles;                                      // page_rows / 16
     FastDiv div_page_tiles, div_units, div_hkv;
     float scale_log2;                                         // log2(e) / sqrt(D)
@@ -279,14 +280,23 @@ struct PackedTiles {
 
 // Where few row blocks meet long contexts, a row block's tokens are shared out among workgroups,
 // every one of which takes the same number of token blocks: the lengths are on the device, so each
-// wave adds up the work of all sequences (a sequence per lane), divides it by the workgroups the
-// launch counts on, and looks up its own piece in the running count.  A launch has a workgroup for
-// every piece of that size and one more for every row block (pieces are rounded up).
-constexpr uint32_t kPackedGroups = 512, kPackedGroupsLog2 = 9;   // workgroups to share out to
+// wave adds up the work of all sequences (a sequence per lane), divides it by the workgroups there is
+// room for, and looks up its own piece in the running count.  Pieces are rounded up, so there may be
+// one more for every row block: where that is the lesser part, the size is chosen for all pieces to
+// run at once (eight drafted trees: 544 pieces of 12 blocks take a second turn on 512 places), else
+// the smaller size evens out the lengths over several turns.
+constexpr uint32_t kPackedGroups = 512;   // two workgroups for each CU
 // Tokens of a piece at the least.  A piece costs a second launch and its sums' way through memory:
 // sixteen sequences of up to 509 cached tokens and one row each (4 KV heads of 64) take 9.3 us on 64
 // workgroups and 12.3 us in pieces of 128.
 constexpr uint32_t kPackedLeastTokens = 512;
+
+// Pieces to divide the work of a KV head into, for `row_blocks` row blocks.  Blocks of many rows leave
+// large parts behind, so they are not divided further than there is room.
+template <uint32_t BM>
+__host__ __device__ constexpr uint32_t packed_room(uint32_t places, uint32_t row_blocks) {
+    return 2 * row_blocks <= places ? places - row_blocks : BM <= 32 && 2 * row_blocks > places ? 2 * row_blocks : places;
+}
 
 struct PackedShare {
     uint32_t s, row_block, piece, pieces, size;   // size: token blocks of a piece
@@ -309,15 +319,21 @@ __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uin
     };
     uint32_t blocks, row_blocks = work(lane, &blocks);
     uint64_t total = (uint64_t)row_blocks * blocks;
+    uint32_t all_rows = row_blocks;
     for (uint32_t s = 64 + lane; s - lane < a.sequences; s += 64) {
         uint32_t more;
         const uint32_t n = work(s, &more);
         total += (uint64_t)n * more;
+        all_rows += n;
     }
 #pragma unroll
-    for (int off = 1; off < 64; off *= 2) total += __shfl_xor((unsigned long long)total, off);
+    for (int off = 1; off < 64; off *= 2) {
+        total += __shfl_xor((unsigned long long)total, off);
+        all_rows += __shfl_xor(all_rows, off);
+    }
     PackedShare p = {};
-    const uint64_t even = (total * a.Hkv + kPackedGroups - 1) >> kPackedGroupsLog2;
+    const uint32_t room = packed_room<BM>(a.places, all_rows);
+    const uint64_t even = total >> 31 ? (total + room - 1) / room : ((uint32_t)total + room - 1) / room;
     constexpr uint32_t least = kPackedLeastTokens / (16 * NT);
     p.size = even > least ? (uint32_t)even : least;
     p.s = ~0u;
@@ -367,7 +383,7 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void sdpa_packed_mfma_kernel(
     const uint32_t team = wave / WQ, member = wave % WQ;
 
     uint32_t s, hkv, rb, piece = 0, pieces = 1, size = 0;
-    if (a.shared_out) {
+    if (a.places) {
         const uint32_t index = divided(blockIdx.x, a.Hkv, a.div_hkv);
         hkv = blockIdx.x - index * a.Hkv;
         const PackedShare share = packed_share<BM, NT>(a, index, false);
@@ -974,7 +990,8 @@ int sdpa_packed_request(int dtype, const iomx_view* q, const iomx_view* k, const
 // How a request runs on the matrix cores: the rows of a block, whether its tokens are shared out,
 // and the workspace the parts need.
 struct PackedPlan {
-    bool mfma, shared_out;
+    bool mfma;
+    uint32_t places;         // see SdpaPackedArgs
     int columns;             // W
     int row_waves;           // WQ
     uint32_t block_rows, row_blocks;
@@ -996,8 +1013,12 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
     // more than one piece.
     const uint64_t capacity = (uint64_t)a.table.cols * a.page_rows + a.max_rows;
     if (p->groups < kPackedGroups && capacity > 2 * kPackedLeastTokens) {
-        p->shared_out = true;
-        p->groups += (kPackedGroups + a.Hkv - 1) / a.Hkv * (uint64_t)a.Hkv;
+        // (few rows of wide heads: a workgroup's stages fill the LDS of a CU)
+        const uint32_t groups = p->row_waves == 1 && a.D > 64 ? kPackedGroups / 2 : kPackedGroups;
+        p->places = (groups + (uint32_t)a.Hkv - 1) / (uint32_t)a.Hkv;
+        // (the row blocks there may be and one more piece for each of packed_room's at the most)
+        const uint64_t most = p->block_rows <= 32 ? 2 * p->groups / a.Hkv : 0;
+        p->groups += (most > p->places ? most : p->places) * a.Hkv;
         p->stats_floats = (p->groups * p->block_rows * 2 + 63) / 64 * 64;
         p->parts_floats = p->groups * p->block_rows * a.D;
     }
@@ -1008,7 +1029,7 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
 template <int DT, int KS, int W, int WQ, int NT>
 void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, hipStream_t st) {
     hipLaunchKernelGGL((sdpa_packed_mfma_kernel<DT, KS, W, 1, WQ, NT>), dim3((uint32_t)p.groups), dim3(256), 0, st, a);
-    if (!p.shared_out) return;
+    if (!p.places) return;
     const uint64_t lanes = (uint64_t)a.max_rows * a.group * (a.D / 4);
     const dim3 joins((uint32_t)((lanes + 255) / 256), a.sequences * a.Hkv);     // fewer than kPackedGroups of them
     hipLaunchKernelGGL((sdpa_packed_join_kernel<DT, W * WQ, NT>), joins, dim3(256), 0, st, a);
@@ -1069,7 +1090,7 @@ extern "C" int iomx_launch_sdpa_packed(int dtype, const iomx_view* q, const iomx
         if (bytes && (!workspace || workspace_bytes < bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
             return IOMX_ERR_INVALID;
         a.row_blocks = p.row_blocks;
-        a.shared_out = p.shared_out;
+        a.places = p.places;
         a.page_tiles = a.page_rows / kTile;
         a.div_page_tiles = make_fast_div(a.page_tiles);
         a.div_units = make_fast_div(a.sequences * a.Hkv);
