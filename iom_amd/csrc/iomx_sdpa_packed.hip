@@ -301,16 +301,18 @@ __host__ __device__ constexpr uint32_t packed_room(uint32_t places, uint32_t row
 struct PackedShare {
     uint32_t s, row_block, piece, pieces, size;   // size: token blocks of a piece
     uint32_t first;                               // index of the sequence's first piece (per KV head)
+    PackedSequence seq;
 };
 
 // The share of piece number `index`, or (find_sequence) of sequence `index`; s = ~0 if there is none.
 template <uint32_t BM, uint32_t NT>
 __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uint32_t index, bool find_sequence) {
     const uint32_t lane = threadIdx.x & 63u;
+    PackedSequence seq = {};
     auto work = [&](uint32_t s, uint32_t* blocks) __attribute__((always_inline)) -> uint32_t {
         *blocks = 0;
         if (s >= a.sequences) return 0;
-        const PackedSequence seq = packed_sequence(a, s);
+        seq = packed_sequence(a, s);
         const uint32_t rows = seq.rows < a.max_rows ? seq.rows : a.max_rows;
         if (!rows) return 0;
         const uint32_t tiles = ((seq.cached + 15) >> 4) + ((seq.start + seq.rows + 15) >> 4) - (seq.start >> 4);
@@ -339,7 +341,7 @@ __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uin
     p.s = ~0u;
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
-        if (s0) row_blocks = work(s0 + lane, &blocks);
+        if (a.sequences > 64) row_blocks = work(s0 + lane, &blocks);
         const uint32_t pieces = (blocks + p.size - 1) / p.size, count = row_blocks * pieces;
         uint32_t upto = count;
 #pragma unroll
@@ -353,6 +355,9 @@ __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uin
             p.s = s0 + at;
             p.pieces = __builtin_amdgcn_readlane(pieces, at);
             p.first = before + __builtin_amdgcn_readlane(upto - count, at);
+            p.seq.start = __builtin_amdgcn_readlane(seq.start, at);
+            p.seq.rows = __builtin_amdgcn_readlane(seq.rows, at);
+            p.seq.cached = __builtin_amdgcn_readlane(seq.cached, at);
             if (!find_sequence) {
                 p.row_block = (index - p.first) / p.pieces;
                 p.piece = index - p.first - p.row_block * p.pieces;
@@ -383,12 +388,14 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void sdpa_packed_mfma_kernel(
     const uint32_t team = wave / WQ, member = wave % WQ;
 
     uint32_t s, hkv, rb, piece = 0, pieces = 1, size = 0;
+    PackedSequence seq;
     if (a.places) {
         const uint32_t index = divided(blockIdx.x, a.Hkv, a.div_hkv);
         hkv = blockIdx.x - index * a.Hkv;
         const PackedShare share = packed_share<BM, NT>(a, index, false);
         if (share.s == ~0u) return;
         s = share.s; rb = share.row_block; piece = share.piece; pieces = share.pieces; size = share.size;
+        seq = share.seq;
     } else {
         // unit (sequence, KV head) fastest: consecutive workgroups go to different dies, a unit's row
         // blocks to the same one where the units are a multiple of eight.  Late rows, which see the
@@ -398,8 +405,8 @@ __global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void sdpa_packed_mfma_kernel(
         rb = a.row_blocks - 1 - rb_up;
         s = divided(unit, a.Hkv, a.div_hkv);
         hkv = unit - s * a.Hkv;
+        seq = packed_sequence(a, s);
     }
-    const PackedSequence seq = packed_sequence(a, s);
     const uint32_t rows = seq.rows < a.max_rows ? seq.rows : a.max_rows;
     const uint32_t m_end = rows * a.group, m_block = rb * BM;
     if (m_block >= m_end) return;
@@ -890,22 +897,43 @@ __global__ __launch_bounds__(256) void sdpa_packed_join_kernel(const SdpaPackedA
     const uint32_t s = divided(blockIdx.y, a.Hkv, a.div_hkv), hkv = blockIdx.y - s * a.Hkv;
     const PackedShare share = packed_share<BM, NT>(a, s, true);
     if (share.pieces <= 1) return;
-    const PackedSequence seq = packed_sequence(a, s);
+    const PackedSequence seq = share.seq;
     const uint32_t rows = seq.rows < a.max_rows ? seq.rows : a.max_rows;
     const uint32_t at = blockIdx.x * 256 + threadIdx.x, m = at / chunks, feature = at % chunks * 4;
     if (m >= rows * a.group) return;
-    // the parts are Hkv workgroups apart
+    // the parts are Hkv workgroups apart; eight of them are on their way together (the last one again
+    // in the place of those past it, with no weight)
     const uint64_t first = ((uint64_t)(share.first + m / BM * share.pieces) * a.Hkv + hkv) * BM + m % BM;
     const uint64_t step = (uint64_t)a.Hkv * BM;
+    constexpr uint32_t kAhead = 8;
+    auto row_of = [&](uint32_t p) { return first + (p < share.pieces ? p : share.pieces - 1) * step; };
     float r = kLowest;
-    for (uint32_t p = 0; p < share.pieces; ++p) r = fmaxf(r, a.part_stats[(first + p * step) * 2]);
+    for (uint32_t p0 = 0; p0 < share.pieces; p0 += kAhead) {
+        float part[kAhead];
+#pragma unroll
+        for (uint32_t n = 0; n < kAhead; ++n) part[n] = a.part_stats[row_of(p0 + n) * 2];
+#pragma unroll
+        for (uint32_t n = 0; n < kAhead; ++n) r = fmaxf(r, part[n]);
+    }
     float l = 0.0f;
     f32x4_t o = {0, 0, 0, 0};
-    for (uint32_t p = 0; p < share.pieces; ++p) {
-        const uint64_t row = first + p * step;
-        const float factor = __builtin_amdgcn_exp2f(a.part_stats[row * 2] - r);
-        l += a.part_stats[row * 2 + 1] * factor;
-        o += *reinterpret_cast<const f32x4_t*>(a.parts + row * a.D + feature) * factor;
+    for (uint32_t p0 = 0; p0 < share.pieces; p0 += kAhead) {
+        float ref[kAhead], sum[kAhead];
+        f32x4_t part[kAhead];
+#pragma unroll
+        for (uint32_t n = 0; n < kAhead; ++n) {
+            const uint64_t row = row_of(p0 + n);
+            ref[n] = a.part_stats[row * 2];
+            sum[n] = a.part_stats[row * 2 + 1];
+            part[n] = *reinterpret_cast<const f32x4_t*>(a.parts + row * a.D + feature);
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < kAhead; ++n) {
+            if (p0 + n >= share.pieces) break;
+            const float factor = __builtin_amdgcn_exp2f(ref[n] - r);
+            l += sum[n] * factor;
+            o += part[n] * factor;
+        }
     }
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
     const uint32_t i = divided(m, a.group, a.div_group), t = seq.start + i;
