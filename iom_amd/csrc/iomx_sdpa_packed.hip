@@ -369,11 +369,19 @@ __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uin
     return p;
 }
 
+// Waves per SIMD: as many workgroups as the stages leave room for in the LDS of a CU, up to two, or
+// three where the registers last (packed prompts of heads of 64 take 167 us with three and 207 us
+// with two).
+constexpr int packed_waves(int KS, int WQ, int NT) {
+    const int fit = 160 * 1024 / (4 * (4 / WQ) * NT * KS * 1024 + 2048), most = KS <= 2 && WQ == 4 ? 3 : 2;
+    return fit < 1 ? 1 : fit < most ? fit : most;
+}
+
 // WQ of the four waves share out the rows of the block and read the same tokens from LDS; the
 // 4 / WQ teams of them share out the tokens.  A wave has QT times W columns; NT token tiles are in
 // LDS per team and stage.
 template <int DT, int KS, int W, int QT, int WQ, int NT>
-__global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void sdpa_packed_mfma_kernel(const SdpaPackedArgs a) {
+__global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfma_kernel(const SdpaPackedArgs a) {
     using Leaf = PackedLeaf<DT>;
     using Shape = PackedShape<DT, KS, W>;
     using Acc = typename Shape::Acc;

@@ -344,3 +344,46 @@ def test_padding_of_the_output_is_left_as_it_was():
     case.run(t=t)
     raw = t["out"].raw().reshape(1, 3, 16, 16)              # 14 rows of 16
     assert (raw[0, :, 14:] == 0x5A5A).all()
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (BF16, 80), (F16, 32)])
+@pytest.mark.parametrize("rows", [4, 8, 16, 32, 33, 70])
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("tree", [False, True])
+def test_every_division_of_the_work(dtype, D, rows, long, tree):
+    """4 query heads on one KV head: 16 rows per KV head and fewer, up to 32, 64, 128 and more, each with
+    contexts whose tokens stay with one workgroup and with ones that are shared out."""
+    ctx = [2300, 0, 700, 1537] if long else [200, 0, 31, 64]
+    case = Attention(50, dtype, (4, 1), D, 64, [rows, 1, rows - 1, rows // 2], ctx, tree=tree, tail=1)
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_more_sequences_than_lanes(dtype):
+    """The shares of 150 sequences, most of them short or without rows."""
+    rng = np.random.default_rng(51)
+    rows = rng.integers(0, 3, 150)
+    ctx = rng.integers(0, 90, 150)
+    ctx[[3, 64, 65, 149]] = [1900, 1500, 1100, 1300]
+    rows[[3, 64, 149]] = [1, 2, 2]
+    case = Attention(51, dtype, (2, 1), 64, 64, list(rows), list(ctx), tail=2)
+    case.check(case.run())
+    case = Attention(52, dtype, (2, 1), 64, 64, [1] * 150, list(ctx))
+    case.check(case.run())
+
+
+def test_a_long_context_of_one_sequence():
+    """A piece for nearly every workgroup, and a context that ends just after a piece."""
+    for ctx in (16384, 9001):
+        case = Attention(53, BF16, (4, 2), 128, 128, [1], [ctx])
+        case.check(case.run())
+        case = Attention(53, F16, (4, 2), 64, 128, [12], [ctx], tree=True)
+        case.check(case.run())
+
+
+def test_a_table_wider_than_the_contexts():
+    """Room for far more pages than there are: the work is divided by the lengths."""
+    case = Attention(54, BF16, (8, 2), 64, 16, [1, 5, 0, 1], [300, 2, 9, 1111])
+    case.table = np.pad(case.table, ((0, 0), (0, 3000)), constant_values=-1)
+    case.M += 3000
+    case.check(case.run())

@@ -174,3 +174,38 @@ def logprobs(dtype=BF16, **kw):
     (dict(dtype=F64), UNSUPPORTED), (dict(dtype=I8), UNSUPPORTED), (dict(dtype=-1), UNSUPPORTED)])
 def test_token_logprobs_refuses(kw, want):
     assert logprobs(**kw) == want
+
+
+def test_attention_needs_its_workspace():
+    views = attention_views(M=64)                    # room for 2048 tokens: their parts are joined
+    rc, nbytes, align = query(views)
+    assert rc == 0 and nbytes > 0 and align == 256
+    aligned = 0x7E0000000000
+    assert launch(views) == INVALID
+    assert launch(views, workspace=aligned, nbytes=nbytes - 1) == INVALID
+    assert launch(views, workspace=aligned + 64, nbytes=nbytes) == INVALID
+    assert query(attention_views(M=4))[1:] == (0, 1)  # 128 tokens stay with their workgroups
+
+
+def test_token_logprobs_needs_its_workspace():
+    views = logprobs_views()
+    nbytes, align = C.c_uint64(0), C.c_uint64(0)
+    assert iomx.lib().iomx_token_logprobs_workspace(BF16, *map(ref, views.values()), C.byref(nbytes), C.byref(align)) == 0
+    assert nbytes.value > 0 and align.value == 256
+    for workspace, given in ((None, 0), (0x7E0000000000, nbytes.value - 1), (0x7E0000000000 + 16, nbytes.value)):
+        assert iomx.lib().iomx_launch_token_logprobs(BF16, *map(ref, views.values()), workspace, given, None) == INVALID
+    assert iomx.lib().iomx_token_logprobs_workspace(BF16, *map(ref, views.values()), None, None) == INVALID
+
+
+def test_borrowed_memory_is_left_alone():
+    """Tensors, buffers and streams of another library: no allocation is made for them, none is freed."""
+    t = iomx.DeviceTensor.at(0x7E0000000000, BF16, (3, 20, 40))
+    assert t.nbytes == 3 * 32 * 48 * 2 and t.view().cview().base == 0x7E0000000000
+    t.free()
+    assert t.view().cview().base is None
+    stream = iomx.Stream.at(0)
+    assert not stream.h
+    stream.close()
+    b = iomx.Buffer.at(0x7E0000000000, 64)
+    b.free()
+    assert not b.ptr
