@@ -33,10 +33,10 @@ struct LogprobsArgs {
 // token_logprobs_scan reads the logits once.  A band (16 rows of a plane) lies in memory as one run
 // of tiles, so a wave's loads are whole kilobytes and a lane meets one row only: lane (row, part of a
 // tile row).  It keeps the row's maximum M, sum e^d and sum d e^d with d = x - M (a difference, not a
-// product with log2 e taken from another: logits near the ends of the range stay finite), 64 or 16
-// logits at a time with the maximum moved before each, and the maximum of every cell of 256 (or 64,
-// or a multiple) columns goes to the workspace.  A few operations and one
-// exponential per logit keep the vector units at about two thirds of what the memory leaves them.
+// product with log2 e taken from another: logits near the ends of the range stay finite), 64,
+// 32 or 16 logits at a time with the maximum moved before each, and the maximum of every cell (a group
+// of 64 to 256 columns, or a few groups) goes to the workspace.  2047 rows of 128256 BF16: 103 us, 5.1
+// TB/s, what a read of as many bytes reaches; the vector units are busy for two thirds of it.
 //
 // token_logprobs_finish, one wave per row, joins the sums and picks the most likely tokens without
 // another pass: a value that K cells' maxima reach is reached by K logits, so only the cells that
@@ -356,13 +356,14 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
         listed += __popcll(there);
         if (ties != ~0u) ties -= __popcll(equal) < ties ? __popcll(equal) : ties;
     }
-    const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 16
+    const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 8 or 16
     {
         __builtin_amdgcn_wave_barrier();       // a wave's LDS operations are in order
-        // A lane takes four columns of a tile; a wave, sixteen tiles: a part of one cell, or four cells.
-        // The loads of eight such pieces are on their way together.
-        constexpr uint32_t kAhead = 8;
-        const uint32_t parts = per_cell < 16 ? 1 : per_cell / 16, together = per_cell < 16 ? 4 : 1;
+        // A lane takes four columns of a tile; a wave, sixteen tiles: a part of one cell, or two or four
+        // cells.  The loads of four such pieces are on their way together (with sixteen the code no
+        // longer fits and a step of 16 rows takes 2 us longer).
+        constexpr uint32_t kAhead = 4;
+        const uint32_t parts = (per_cell + 15) / 16, together = per_cell < 16 ? 16 / per_cell : 1;
         const uint32_t pieces = (listed + together - 1) / together * parts;
         for (uint32_t p0 = 0; p0 < pieces && count <= kMostCandidates; p0 += kAhead) {
             float x[kAhead][4];
@@ -370,11 +371,11 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
 #pragma unroll
             for (uint32_t n = 0; n < kAhead; ++n) {
                 const uint32_t p = p0 + n;
-                const uint32_t entry = together == 4 ? p * 4 + (lane >> 4) : p / parts;
-                const uint32_t tile_in_cell = together == 4 ? (lane >> 2) & 3u : p % parts * 16 + (lane >> 2);
+                const uint32_t entry = together > 1 ? p * together + (lane >> 2) / per_cell : p / parts;
+                const uint32_t tile_in_cell = together > 1 ? (lane >> 2) % per_cell : p % parts * 16 + (lane >> 2);
                 const uint32_t tile = (entry < listed ? chosen[wave][entry] : 0u) * per_cell + tile_in_cell;
                 first[n] = tile * kTile + (lane & 3u) * 4;
-                const bool in = p < pieces && entry < listed && tile < a.tile_cols;
+                const bool in = p < pieces && entry < listed && tile_in_cell < per_cell && tile < a.tile_cols;
                 // a tile's padding columns are read with it, and not looked at
                 const uint8_t* at = row + ((uint64_t)(in ? tile : 0u) * kTileSlots + (lane & 3u) * 4) * kSize;
                 if constexpr (DT == IOMX_DT_F32) {
@@ -520,11 +521,16 @@ int logprobs_request(int dtype, const iomx_view* logits, const iomx_view* tokens
     return IOMX_OK;
 }
 
+template <int DT> constexpr int kWideGroup = DT == IOMX_DT_F32 ? 16 : 8;
+
 // The scan's layout, and the floats of workspace it takes.
-int logprobs_layout(LogprobsArgs* a, uint64_t* stats_floats, uint64_t* cell_floats) {
-    // groups of 64 columns for small vocabularies, so that even a row of few thousand logits has a
-    // cell for each of the K most likely; cells of several groups where there would be too many
-    a->group_tiles = a->V < 16384 ? 4 : 16;
+int logprobs_layout(int dtype, LogprobsArgs* a, uint64_t* stats_floats, uint64_t* cell_floats) {
+    // Groups of 64 columns for small vocabularies, so that even a row of few thousand logits has a
+    // cell for each of the K most likely; cells of several groups where there would be too many.
+    // Larger groups are 4 KiB of the 16-bit leaves and 16 KiB of F32 for a wave: 2047 rows of 128256
+    // BF16 scan in 103 us with 8 tiles and in 116 us with 16 (half the waves for the registers), 333
+    // rows of 50257 F32 in 18.7 us with 8 and 16.2 us with 16 (a wave has one or two groups).
+    a->group_tiles = a->V < 16384 ? 4 : dtype == IOMX_DT_F32 ? kWideGroup<IOMX_DT_F32> : kWideGroup<IOMX_DT_BF16>;
     const uint32_t groups = (a->tile_cols + a->group_tiles - 1) / a->group_tiles;
     a->cell_groups = (groups + kMostCells - 1) / kMostCells;
     a->cells = (groups + a->cell_groups - 1) / a->cell_groups;
@@ -547,8 +553,8 @@ void launch_logprobs(const LogprobsArgs& a, hipStream_t st) {
     const dim3 grid((uint32_t)(a.walk.planes * a.bands * a.splits));
     if (a.group_tiles == 4 && a.entropy) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 4, true>), grid, dim3(256), 0, st, a);
     else if (a.group_tiles == 4) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 4, false>), grid, dim3(256), 0, st, a);
-    else if (a.entropy) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 16, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 16, false>), grid, dim3(256), 0, st, a);
+    else if (a.entropy) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, kWideGroup<DT>, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, kWideGroup<DT>, false>), grid, dim3(256), 0, st, a);
     hipLaunchKernelGGL(token_logprobs_finish_kernel<DT>, dim3((a.rows + 3) / 4), dim3(256), 0, st, a);
     record_launch("token_logprobs", grid.x, 256, (uint64_t)a.rows * a.V);
 }
@@ -567,7 +573,7 @@ extern "C" int iomx_token_logprobs_workspace(int dtype, const iomx_view* logits,
     LogprobsArgs a = {};
     IOMX_TRY(logprobs_request(dtype, logits, tokens, logprobs, entropy, top_ids, top_logprobs, &a));
     uint64_t stats, cells;
-    IOMX_TRY(logprobs_layout(&a, &stats, &cells));
+    IOMX_TRY(logprobs_layout(dtype, &a, &stats, &cells));
     *bytes = (stats + cells) * 4;
     *alignment = 256;
     return IOMX_OK;
@@ -580,7 +586,7 @@ extern "C" int iomx_launch_token_logprobs(int dtype, const iomx_view* logits, co
     LogprobsArgs a = {};
     IOMX_TRY(logprobs_request(dtype, logits, tokens, logprobs, entropy, top_ids, top_logprobs, &a));
     uint64_t stats, cells;
-    IOMX_TRY(logprobs_layout(&a, &stats, &cells));
+    IOMX_TRY(logprobs_layout(dtype, &a, &stats, &cells));
     if (!workspace || workspace_bytes < (stats + cells) * 4 || (reinterpret_cast<uintptr_t>(workspace) & 255u))
         return IOMX_ERR_INVALID;
     a.stats = static_cast<float*>(workspace);

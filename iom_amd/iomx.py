@@ -177,13 +177,14 @@ def lib() -> C.CDLL:
         l.iomx_launch_scatter.argtypes = [C.c_int, VP, P, P]
         l.iomx_launch_gather.argtypes = [C.c_int, VP, P, P]
         l.iomx_launch_softmax.argtypes = [C.POINTER(SoftmaxDesc), P]
+        # (views as plain addresses: see _refs)
         U64P = C.POINTER(C.c_uint64)
-        l.iomx_sdpa_packed_workspace.argtypes = [C.c_int] + [VP] * 10 + [C.c_uint64, U64P, U64P]
-        l.iomx_launch_sdpa_packed.argtypes = [C.c_int] + [VP] * 10 + [C.c_uint64, P, C.c_uint64, C.c_int, P]
-        l.iomx_launch_rope_packed.argtypes = [C.c_int, VP, VP, VP, C.c_double, P]
-        l.iomx_launch_cache_append_packed.argtypes = [C.c_int] + [VP] * 8 + [P]
-        l.iomx_token_logprobs_workspace.argtypes = [C.c_int] + [VP] * 6 + [U64P, U64P]
-        l.iomx_launch_token_logprobs.argtypes = [C.c_int] + [VP] * 6 + [P, C.c_uint64, P]
+        l.iomx_sdpa_packed_workspace.argtypes = [C.c_int] + [P] * 10 + [C.c_uint64, U64P, U64P]
+        l.iomx_launch_sdpa_packed.argtypes = [C.c_int] + [P] * 10 + [C.c_uint64, P, C.c_uint64, C.c_int, P]
+        l.iomx_launch_rope_packed.argtypes = [C.c_int, P, P, P, C.c_double, P]
+        l.iomx_launch_cache_append_packed.argtypes = [C.c_int] + [P] * 9
+        l.iomx_token_logprobs_workspace.argtypes = [C.c_int] + [P] * 6 + [U64P, U64P]
+        l.iomx_launch_token_logprobs.argtypes = [C.c_int] + [P] * 7 + [C.c_uint64, P]
         l.iomx_last_launch.argtypes = [C.POINTER(LaunchInfo)]
         _lib = l
     return _lib
@@ -421,7 +422,7 @@ class DeviceView:
         self.dims = tuple(int(d) for d in dims)
         self.plane_offset = int(plane_offset)
         self.plane_strides = tuple(int(s) for s in plane_strides)
-        self._held = None   # (C struct, reference to it): see ref()
+        self._held = None   # (C struct, its address): see _refs()
 
     @property
     def dtype(self):
@@ -477,15 +478,10 @@ class DeviceView:
             v.plane_strides[i] = s
         return v
 
-    def ref(self):
-        """The view as a C argument: one struct per DeviceView, built on the first use (a struct
-        per call costs more than the rest of a small launch)."""
-        if self._held is None:
-            view = self.cview()
-            self._held = view, C.byref(view)
-        view, reference = self._held
-        view.base = self.owner.buf.ptr.value     # a freed owner is a null pointer, which is refused
-        return reference
+    def _hold(self):
+        view = self.cview()
+        self._held = view, C.addressof(view)
+        return self._held
 
     @property
     def logical_count(self) -> int:
@@ -648,8 +644,18 @@ def rope(x: DeviceView, out: DeviceView, a: int, theta: float, stream: Optional[
 
 
 def _refs(*views: Optional[DeviceView]):
-    """A C argument for each view; None is a null pointer."""
-    return [None if v is None else v.ref() for v in views]
+    """A C argument for each view; None is a null pointer.  A view's struct is built once, on its first
+    use (ten structs for a call cost more than a small launch); the address of the storage is looked
+    up every time, so that a freed owner is a null pointer, which is refused."""
+    refs = []
+    for v in views:
+        if v is None:
+            refs.append(None)
+            continue
+        struct, address = v._held or v._hold()
+        struct.base = v.owner.buf.ptr.value
+        refs.append(address)
+    return refs
 
 
 def _queried(call, *args):
