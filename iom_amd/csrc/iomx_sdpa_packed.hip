@@ -211,6 +211,7 @@ template <> struct PackedLeaf<IOMX_DT_F16> {
 };
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4_t* tr_ptr_t;
 
 // Sixteen lanes read 128 consecutive bytes, four rows of a tile of 16-bit elements; lane i of them
@@ -337,7 +338,8 @@ __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uin
     const uint32_t room = packed_room<BM>(a.places, all_rows);
     const uint64_t even = total >> 31 ? (total + room - 1) / room : ((uint32_t)total + room - 1) / room;
     constexpr uint32_t least = kPackedLeastTokens / (16 * NT);
-    p.size = even > least ? (uint32_t)even : least;
+    // (the same in every lane, and known to be: what is formed from it goes to the scalar unit)
+    p.size = __builtin_amdgcn_readfirstlane(even > least ? (uint32_t)even : least);
     p.s = ~0u;
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
@@ -475,13 +477,16 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     // block's turn (present_of): a comparison here would wait for the load, and with it for every
     // tile on its way to LDS.
     auto block_pages = [&](uint32_t b) __attribute__((always_inline)) -> uint32_t {
+        if (b >= b_end || b * NT >= tiles.prefix) return 0u;
         const uint32_t x = b * NT + lane;
-        if (lane >= NT || b >= b_end || x >= tiles.prefix) return 0u;
+        if (lane >= NT || x >= tiles.prefix) return 0u;
         return (uint32_t)a.table.at(s, divided(x, a.page_tiles, a.div_page_tiles));
     };
     auto present_of = [&](uint32_t b, uint32_t pages) __attribute__((always_inline)) -> uint32_t {
+        if (b >= b_end) return 0u;
+        if (b * NT >= tiles.prefix) return tiles.count - b * NT >= NT ? (1u << NT) - 1u : (1u << (tiles.count - b * NT)) - 1u;
         const uint32_t x = b * NT + lane;
-        return (uint32_t)__ballot(lane < NT && b < b_end && x < tiles.count && (x >= tiles.prefix || pages < a.pages));
+        return (uint32_t)__ballot(lane < NT && x < tiles.count && (x >= tiles.prefix || pages < a.pages));
     };
     // brings the tiles of block b that are present to a stage: a wave of the team takes every WQ-th
     auto fetch = [&](uint32_t b, uint32_t pages, uint32_t present, uint8_t* ks, uint8_t* vs) __attribute__((always_inline)) {
@@ -590,16 +595,20 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     auto words = [&](uint32_t (&w)[2 * QUADS], int h) __attribute__((always_inline)) {
         return u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
     };
-    // A block that every row of the wave sees in full and whose scores are below the references; false
-    // if they are not (nothing is changed then: any_pair takes the block, and the sums, which only it
-    // scales, keep their registers here).
+    // A block that every row of the wave sees in full and whose scores are below the references, which
+    // the wave's first block sets; false if they are not (nothing is changed then: any_pair takes the
+    // block, and the sums, which only it scales, keep their registers here).
+    bool begun = false;
     auto whole_block = [&](const uint8_t* ks, const uint8_t* vs) __attribute__((always_inline)) -> bool {
         Acc sc[NT / 2][QT][Shape::kScores];
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) scores(ks + n * (2 * KS * 1024), sc[n]);
         float top[QT];
         largest(sc, top);
-        if (beyond(top)) return false;
+        if (!begun) {
+#pragma unroll
+            for (int q = 0; q < QT; ++q) ref[q] = fmaxf(Shape::join(top[q]), kLowest);
+        } else if (beyond(top)) return false;
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) {
             uint32_t pw[QT][2 * QUADS];
@@ -623,6 +632,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
         scores(ks, sc[0]);
         uint32_t seen[QT];                  // bit 4 u + j: the column sees token j of quad u
         uint32_t keep[2 * QUADS];           // V words (two tokens each) that some row may see
+        bool ragged = false;                // there are tokens that none may see
         if (!whole) {
 #pragma unroll
             for (int q = 0; q < QT; ++q) seen[q] = 0;
@@ -662,6 +672,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
                         }
                     }
                 }
+                ragged = ragged || any != 0xFFFFu;
 #pragma unroll
                 for (int u = 0; u < QUADS; ++u) {
                     if (Shape::quad_tile(u) != t) continue;
@@ -705,16 +716,20 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
 #pragma unroll
             for (int d = 0; d < Shape::kAccs; ++d) vf[d] = values(vs, d, h);
             if (!whole) {
-                // the sign bits of `wild`: some exponent field is all ones
-                uint32_t wild = 0;
+                if (ragged) {
+#pragma unroll
+                    for (int d = 0; d < Shape::kAccs; ++d)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) vf[d][w] &= keep[4 * h + w];
+                }
+                // the largest magnitude of each half: an exponent field of all ones is above every other
+                u16x2_t wild = {0, 0};
 #pragma unroll
                 for (int d = 0; d < Shape::kAccs; ++d)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        vf[d][w] &= keep[4 * h + w];
-                        wild |= (vf[d][w] & 0x7FFF7FFFu) + (Leaf::kCarry | Leaf::kCarry << 16);
-                    }
-                if (__any((wild & 0x80008000u) != 0)) {
+                    for (int w = 0; w < 4; ++w)
+                        wild = __builtin_elementwise_max(wild, __builtin_bit_cast(u16x2_t, vf[d][w] & 0x7FFF7FFFu));
+                if (__any(wild.x >= Leaf::kExponent || wild.y >= Leaf::kExponent)) {
 #pragma unroll
                     for (int q = 0; q < QT; ++q) {
                         u32x4 ones;
@@ -784,9 +799,11 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
         if constexpr (decltype(stage)::value) { ks = &k_odd[team][0]; vs = &v_odd[team][0]; }
         else { ks = &k_even[team][0]; vs = &v_even[team][0]; }
         const uint32_t x = b * NT;
-        // (the first block sets the references)
-        if (here == (1u << NT) - 1u && (x + NT <= whole_prefix || (x >= whole_first && x + NT <= whole_end))
-            && b >= b_begin + WK && whole_block(ks, vs)) return;
+        if (here == (1u << NT) - 1u && (x + NT <= whole_prefix || (x >= whole_first && x + NT <= whole_end)) && whole_block(ks, vs)) {
+            begun = true;
+            return;
+        }
+        begun = true;
 #pragma unroll 1
         for (uint32_t n = 0; n < NT / 2; ++n)
             any_pair(x + 2 * n, (here >> (2 * n)) & 3u, ks + n * 2 * KS * 1024, vs + n * 2 * KS * 1024);
