@@ -233,6 +233,9 @@ template <int DT, int KS> struct PackedShape<DT, KS, 16> {
     // feature tile and byte within its row that a lane supplies in step c
     static __device__ __forceinline__ uint32_t operand_tile(int c, uint32_t lane) { return 2 * c + (lane >> 5); }
     static __device__ __forceinline__ uint32_t operand_byte(uint32_t lane) { return ((lane >> 4) & 1u) * 16; }
+    // sixteen-byte piece of a kilobyte that a lane of the loader brings
+    static __device__ __forceinline__ uint32_t k_source(uint32_t lane, uint32_t) { return lane; }
+    static __device__ __forceinline__ uint32_t v_source(uint32_t lane) { return lane; }
     // first operand of S^T: byte within the pair's stage, score tile t, step c
     static __device__ __forceinline__ uint32_t k_lane(uint32_t lane) { return (lane >> 5) * kTile16 + (lane & 15u) * 32 + operand_byte(lane); }
     static constexpr int k_at(int t, int c) { return t * KS * 1024 + c * 1024; }
@@ -258,12 +261,23 @@ template <int DT, int KS> struct PackedShape<DT, KS, 32> {
     static __device__ __forceinline__ uint32_t column(uint32_t lane) { return lane & 31u; }
     static __device__ __forceinline__ uint32_t operand_tile(int c, uint32_t) { return c; }
     static __device__ __forceinline__ uint32_t operand_byte(uint32_t lane) { return (lane >> 5) * 16; }
-    static __device__ __forceinline__ uint32_t k_lane(uint32_t lane) { return ((lane >> 4) & 1u) * (KS * 1024) + (lane & 15u) * 32 + operand_byte(lane); }
+    // The two token tiles of a pair would be read from the same banks at once, as would two feature
+    // tiles of V: the second of either lies in LDS with its rows' halves, or its runs of four rows,
+    // exchanged (a lane of the loader may take its sixteen bytes from anywhere).
+    static __device__ __forceinline__ uint32_t k_source(uint32_t lane, uint32_t token_tile) { return lane ^ (token_tile & 1u); }
+    static __device__ __forceinline__ uint32_t v_source(uint32_t lane) { return lane ^ (lane >> 5) * 8; }
+    static __device__ __forceinline__ uint32_t k_lane(uint32_t lane) {
+        const uint32_t second = (lane >> 4) & 1u;
+        return second * (KS * 1024) + (lane & 15u) * 32 + ((lane >> 5) ^ second) * 16;
+    }
     static constexpr int k_at(int, int c) { return c * 512; }
     static constexpr int quad_tile(int u) { return u >> 1; }
     static __device__ __forceinline__ uint32_t quad_run(int u, uint32_t lane) { return 2 * (u & 1) + (lane >> 5); }
     // sixteen tokens (tile h) of feature tiles 2 d and 2 d + 1
-    static __device__ __forceinline__ uint32_t v_lane(uint32_t lane) { return ((lane >> 4) & 1u) * 512 + (lane >> 5) * 128 + (lane & 15u) * 8; }
+    static __device__ __forceinline__ uint32_t v_lane(uint32_t lane) {
+        const uint32_t second = (lane >> 4) & 1u;
+        return second * 512 + ((lane >> 5) ^ second) * 128 + (lane & 15u) * 8;
+    }
     static constexpr int v_at(int d, int h, int part) { return h * KS * 1024 + d * 1024 + part * 256; }
     static constexpr int v_quad(int h, int part) { return 2 * h + part; }
     static __device__ __forceinline__ uint32_t feature(int d, int u, uint32_t lane) { return 32 * d + 8 * u + 4 * (lane >> 5); }
@@ -490,6 +504,10 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     };
     // brings the tiles of block b that are present to a stage: a wave of the team takes every WQ-th
     auto fetch = [&](uint32_t b, uint32_t pages, uint32_t present, uint8_t* ks, uint8_t* vs) __attribute__((always_inline)) {
+        // (where registers are scarce, not to be known as the same lane every time: the addresses formed
+        // from it would be kept in registers throughout the loop)
+        uint32_t own_lane = lane;
+        if constexpr (packed_waves(KS, WQ, NT) == 3) asm volatile("" : "+v"(own_lane));
 #pragma unroll
         for (int n = 0; n < NT / WQ; ++n) {
             const uint32_t at = member + n * WQ;
@@ -510,8 +528,8 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
                 if (c == KS - 1 && odd && lane >= 32) break;
-                __builtin_amdgcn_global_load_lds((gptr_t)(kt + c * 1024 + lane * 16), (lptr_t)(ks + at * (KS * 1024) + c * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((gptr_t)(vt + c * 1024 + lane * 16), (lptr_t)(vs + at * (KS * 1024) + c * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((gptr_t)(kt + c * 1024 + Shape::k_source(own_lane, at) * 16), (lptr_t)(ks + at * (KS * 1024) + c * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((gptr_t)(vt + c * 1024 + Shape::v_source(own_lane) * 16), (lptr_t)(vs + at * (KS * 1024) + c * 1024), 16, 0, 0);
             }
         }
     };
@@ -659,7 +677,8 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
                         for (int q = 0; q < QT; ++q) {
                             if (a.tree.base) {
                                 if (m_wave + W * q + column < m_end) {
-                                    const uint32_t row = seq.start + row_of[q];
+                                    uint32_t row = seq.start + row_of[q];
+                                    if constexpr (packed_waves(KS, WQ, NT) == 3) asm volatile("" : "+v"(row));   // (as in fetch)
                                     const int32_t w = j >> 5;              // -1 for the rows before the first
                                     const uint32_t lo = w >= 0 && w < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w) : 0u;
                                     const uint32_t hi = w + 1 < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w + 1) : 0u;
@@ -740,24 +759,22 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
                         }
 #pragma unroll
                         for (int d = 0; d < Shape::kAccs; ++d) {
-                            u32x4 plus, minus;
+#pragma unroll 1
+                            for (uint32_t sign = 0; sign < 2; ++sign) {
+                                u32x4 special;
 #pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                uint32_t up = 0, down = 0;
+                                for (int w = 0; w < 4; ++w) {
+                                    special[w] = 0;
 #pragma unroll
-                                for (int half = 0; half < 32; half += 16) {
-                                    const uint32_t e = vf[d][w] >> half & 0x7FFFu, negative = vf[d][w] >> half & 0x8000u;
-                                    up |= (e > Leaf::kExponent || (e == Leaf::kExponent && !negative) ? Leaf::kOne : 0u) << half;
-                                    down |= (e > Leaf::kExponent || (e == Leaf::kExponent && negative) ? Leaf::kOne : 0u) << half;
+                                    for (int half = 0; half < 32; half += 16) {
+                                        const uint32_t e = vf[d][w] >> half & 0xFFFFu, size = e & 0x7FFFu;
+                                        special[w] |= (size > Leaf::kExponent || (size == Leaf::kExponent && e >> 15 == sign) ? Leaf::kOne : 0u) << half;
+                                    }
                                 }
-                                plus[w] = up;
-                                minus[w] = down;
-                            }
-                            const Acc n = Leaf::mfma(plus, ones, Acc{}), m = Leaf::mfma(minus, ones, Acc{});
+                                const Acc n = Leaf::mfma(special, ones, Acc{});
 #pragma unroll
-                            for (int j = 0; j < 4 * Shape::kAccQuads; ++j) {
-                                if (n[j] > 0.0f) acc[d][q][j] += __builtin_inff();
-                                if (m[j] > 0.0f) acc[d][q][j] -= __builtin_inff();
+                                for (int j = 0; j < 4 * Shape::kAccQuads; ++j)
+                                    if (n[j] > 0.0f) acc[d][q][j] += sign ? -__builtin_inff() : __builtin_inff();
                             }
                         }
                     }
