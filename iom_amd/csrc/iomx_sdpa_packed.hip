@@ -310,7 +310,7 @@ constexpr uint32_t kPackedLeastTokens = 512;
 // large parts behind, so they are not divided further than there is room.
 template <uint32_t BM>
 __host__ __device__ constexpr uint32_t packed_room(uint32_t places, uint32_t row_blocks) {
-    return 2 * row_blocks <= places ? places - row_blocks : BM <= 32 && 2 * row_blocks > places ? 2 * row_blocks : places;
+    return 2 * row_blocks <= places ? places - row_blocks : BM <= 32 ? 2 * row_blocks : places;
 }
 
 struct PackedShare {
@@ -1079,10 +1079,12 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
     p->block_rows = (uint32_t)(p->columns * p->row_waves);
     p->row_blocks = (uint32_t)((m + p->block_rows - 1) / p->block_rows);
     p->groups = (uint64_t)a.sequences * a.Hkv * p->row_blocks;
-    // Shared out where there are fewer row blocks than two per CU and a sequence may have tokens for
-    // more than one piece.
+    // Shared out where there are few row blocks and a sequence may have tokens for more than one piece:
+    // fewer than two per CU, or than one where a block has many rows and leaves large parts behind (128
+    // blocks of four trees of 128 rows: 58 us shared out, 119 us not; 376 blocks of a prompt of 1500 rows,
+    // 4 KV heads of 64: 50 us shared out, 33 us not).
     const uint64_t capacity = (uint64_t)a.table.cols * a.page_rows + a.max_rows;
-    if (p->groups < kPackedGroups && capacity > 2 * kPackedLeastTokens) {
+    if (p->groups < (p->block_rows <= 32 ? kPackedGroups : kPackedGroups / 2) && capacity > 2 * kPackedLeastTokens) {
         // (few rows of wide heads: a workgroup's stages fill the LDS of a CU)
         const uint32_t groups = p->row_waves == 1 && a.D > 64 ? kPackedGroups / 2 : kPackedGroups;
         p->places = (groups + (uint32_t)a.Hkv - 1) / (uint32_t)a.Hkv;
