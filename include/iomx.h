@@ -430,7 +430,9 @@ int iomx_launch_softmax(const iomx_softmax_desc* desc, iomx_stream_t stream);
  * unnormalised probabilities are rounded to the leaf on the matrix cores, one rounding at
  * the store.  A row that sees nothing, or only scores of -inf, is +0; one that sees a NaN
  * or a score of +inf is NaN.  Rows of no sequence are left as they were; `max_rows` is the
- * caller's bound on starts[s+1] - starts[s], and rows past it are left as they were too.
+ * caller's bound on starts[s+1] - starts[s], and rows past it are left as they were too (the
+ * launch has workgroups for max_rows rows of every sequence: a tight bound, 1 in a step of
+ * single tokens, picks the right kernel).
  *
  * path 0 picks the kernel: the matrix cores where D % 16 == 0, D <= 128 and P % 16 == 0,
  * else one wave per row and head; path 1 forces the latter (tests).

@@ -46,6 +46,9 @@ struct LogprobsArgs {
 
 constexpr uint32_t kMostCells = 512;          // of a row: eight per lane
 constexpr uint32_t kMostChosen = 256;         // cells that are read again
+// Logits of a row that a wave holds: up to here they are their own cells, since with no more cells than places
+// nearly every logit is above the bound (686 logits, their 20 most likely: 55 us by cells of 64, 20 us by logits).
+constexpr uint32_t kSmall = 2560;
 constexpr uint32_t kMostCandidates = 128;     // of a row: two per lane
 
 // d as a factor of e^d: from -200 on down e^d is 0 in F32, and its product with d is, too
@@ -223,11 +226,13 @@ __device__ __forceinline__ float wave_sum(float x) {
     return wave_reduce(x, [](float a, float b) { return a + b; });
 }
 
-template <int DT>
+// SMALL: a vocabulary of at most kSmall tokens, whose logits are their own cells.
+template <int DT, bool SMALL>
 __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const LogprobsArgs a) {
     constexpr int kSize = DT == IOMX_DT_F32 ? 4 : 2;
     constexpr float inf = __builtin_inff();
-    constexpr uint32_t kSlots = kMostCells / 64;
+    constexpr uint32_t kSlots = (SMALL ? kSmall : kMostCells) / 64, kMostListed = SMALL ? kMostCandidates : kMostChosen;
+    const uint32_t all_cells = SMALL ? a.V : a.cells;
     __shared__ uint64_t found[4][kMostCandidates];
     __shared__ uint16_t chosen[4][kMostChosen];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -246,7 +251,8 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i) {
             const uint32_t c = i * 64 + lane;
-            cells[i] = c < a.cells ? maxima[(uint64_t)c * kTile] : -inf;
+            if constexpr (SMALL) cells[i] = c < a.V ? logit_at<DT>(row, c) : -inf;
+            else cells[i] = c < a.cells ? maxima[(uint64_t)c * kTile] : -inf;
         }
     }
     // ... and the splits' sums, one per lane (there are 64 at the most)
@@ -299,7 +305,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
         uint32_t n = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i)
-            if (i * 64 < a.cells) n += __popcll(__ballot(cells[i] >= bound));
+            if (i * 64 < all_cells) n += __popcll(__ballot(cells[i] >= bound));
         return n;
     };
     auto largest_below = [&](float limit) __attribute__((always_inline)) -> float {
@@ -308,56 +314,58 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
         for (uint32_t i = 0; i < kSlots; ++i) top = fmaxf(top, cells[i] < limit ? cells[i] : -inf);
         return wave_max(top);
     };
-    float bound = -inf;
-    uint32_t reached = 0, ties = ~0u;              // ties: cells of exactly the bound that are looked at
-    if (a.cells >= a.K) {
-        const float top = largest_below(inf);
-        float over = top, step = fmaxf(1.0f, fabsf(top) * 0.0078125f);   // `over`: fewer than K reach it, or it is the top
-        for (;;) {
-            bound = top - step;
-            reached = reaching(bound);
-            if (reached >= a.K || bound == -inf) break;
-            over = bound;
-            step *= 2.0f;
-        }
-        for (int halvings = 0; halvings < 12 && reached > a.K + a.K / 2; ++halvings) {
-            const float middle = bound + (over - bound) * 0.5f;
-            const uint32_t n = reaching(middle);
-            if (n >= a.K) { bound = middle; reached = n; }
-            else over = middle;
-        }
-        if (bound > -inf && reached > kMostChosen) {
-            // (rows of equal logits) the K-th largest maximum itself: of the cells that have it, those
-            // with the lowest columns make up the K cells that hold the K most likely tokens
-            uint32_t larger = 0;
-            bound = top;
-            for (;;) {
-                uint32_t equal = 0;
-#pragma unroll
-                for (uint32_t i = 0; i < kSlots; ++i) equal += __popcll(__ballot(cells[i] == bound));
-                if (larger + equal >= a.K) break;
-                larger += equal;
-                bound = largest_below(bound);
-            }
-            ties = a.K - larger;
-        }
+    uint32_t ties = ~0u;                           // cells of exactly the bound that are looked at
+    const float top = largest_below(inf);
+    float over = top, step = fmaxf(1.0f, fabsf(top) * 0.0078125f);   // `over`: fewer than K reach it, or it is the top
+    float bound;
+    uint32_t reached;
+    for (;;) {
+        bound = fmaxf(top - step, -3.4028234663852886e38f);          // that one: every finite logit
+        reached = reaching(bound);
+        if (reached >= a.K || bound == -3.4028234663852886e38f) break;
+        over = bound;
+        step *= 2.0f;
     }
-    // fewer than K cells, or than K with a finite maximum: every finite logit
-    if (bound == -inf) bound = -3.4028234663852886e38f;
+    // (of few cells nearly all would be taken, and far more logits with them)
+    const uint32_t spare = (all_cells - a.K) / 4, enough = a.K + (spare < a.K / 2 ? spare : a.K / 2);
+    for (int halvings = 0; halvings < 12 && reached > enough; ++halvings) {
+        const float middle = bound * 0.5f + over * 0.5f;
+        const uint32_t n = reaching(middle);
+        if (n >= a.K) { bound = middle; reached = n; }
+        else over = middle;
+    }
+    if (reached > kMostListed) {
+        // (rows of equal logits) the K-th largest maximum itself: of the cells that have it, those
+        // with the lowest columns make up the K cells that hold the K most likely tokens
+        uint32_t larger = 0;
+        bound = top;
+        for (;;) {
+            uint32_t equal = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) equal += __popcll(__ballot(cells[i] == bound));
+            if (larger + equal >= a.K) break;
+            larger += equal;
+            bound = largest_below(bound);
+        }
+        ties = a.K - larger;
+    }
     // the logits that reach it
     uint32_t count = 0, listed = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kSlots; ++i) {
-        if (i * 64 >= a.cells) break;
+        if (i * 64 >= all_cells) break;
         const uint64_t below = (1ull << lane) - 1, equal = __ballot(cells[i] == bound);
         const bool take = cells[i] > bound || (cells[i] == bound && (uint32_t)__popcll(equal & below) < ties);
         const uint64_t there = __ballot(take);
-        if (take) chosen[wave][listed + __popcll(there & below)] = (uint16_t)(i * 64 + lane);
+        const uint32_t place = listed + __popcll(there & below);
+        if constexpr (SMALL) { if (take) found[wave][place] = top_key(cells[i], i * 64 + lane); }
+        else if (take) chosen[wave][place] = (uint16_t)(i * 64 + lane);
         listed += __popcll(there);
         if (ties != ~0u) ties -= __popcll(equal) < ties ? __popcll(equal) : ties;
     }
     const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 8 or 16
-    {
+    if constexpr (SMALL) count = listed;
+    else {
         __builtin_amdgcn_wave_barrier();       // a wave's LDS operations are in order
         // A lane takes four columns of a tile; a wave, sixteen tiles: a part of one cell, or two or four
         // cells.  The loads of four such pieces are on their way together (with sixteen the code no
@@ -403,7 +411,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
                 }
         }
     }
-    if (count <= kMostCandidates) {
+    if (SMALL || count <= kMostCandidates) {
         __builtin_amdgcn_wave_barrier();
         const uint64_t one = lane < count ? found[wave][lane] : 0, two = lane + 64 < count ? found[wave][lane + 64] : 0;
         uint32_t before_one = 0, before_two = 0;
@@ -526,7 +534,7 @@ template <int DT> constexpr int kWideGroup = DT == IOMX_DT_F32 ? 16 : 8;
 // The scan's layout, and the floats of workspace it takes.
 int logprobs_layout(int dtype, LogprobsArgs* a, uint64_t* stats_floats, uint64_t* cell_floats) {
     // Groups of 64 columns for small vocabularies, so that even a row of few thousand logits has a
-    // cell for each of the K most likely; cells of several groups where there would be too many.
+    // cell for each of the K most likely and a few more; cells of several groups where there would be too many.
     // Larger groups are 4 KiB of the 16-bit leaves and 16 KiB of F32 for a wave: 2047 rows of 128256
     // BF16 scan in 103 us with 8 tiles and in 116 us with 16 (half the waves for the registers), 333
     // rows of 50257 F32 in 18.7 us with 8 and 16.2 us with 16 (a wave has one or two groups).
@@ -544,7 +552,7 @@ int logprobs_layout(int dtype, LogprobsArgs* a, uint64_t* stats_floats, uint64_t
     a->div_splits = make_fast_div(a->splits);
     if (bands * a->splits > 0x7FFFFFF0ull) return IOMX_ERR_OVERFLOW;
     *stats_floats = bands * a->splits * kTile * 4;
-    *cell_floats = a->top_ids ? bands * a->cells * kTile : 0;
+    *cell_floats = a->top_ids && a->V > kSmall ? bands * a->cells * kTile : 0;
     return IOMX_OK;
 }
 
@@ -555,7 +563,9 @@ void launch_logprobs(const LogprobsArgs& a, hipStream_t st) {
     else if (a.group_tiles == 4) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 4, false>), grid, dim3(256), 0, st, a);
     else if (a.entropy) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, kWideGroup<DT>, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, kWideGroup<DT>, false>), grid, dim3(256), 0, st, a);
-    hipLaunchKernelGGL(token_logprobs_finish_kernel<DT>, dim3((a.rows + 3) / 4), dim3(256), 0, st, a);
+    const dim3 rows((a.rows + 3) / 4);
+    if (a.V <= kSmall) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, true>), rows, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, false>), rows, dim3(256), 0, st, a);
     record_launch("token_logprobs", grid.x, 256, (uint64_t)a.rows * a.V);
 }
 

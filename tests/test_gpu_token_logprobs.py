@@ -89,6 +89,9 @@ def run(dtype, raw, tokens=None, K=0, entropy=True, lead_view=None):
 
 
 def close(got, want, far, what):
+    # F32 ends at (2 - 2^-23) 2^127: what lies half a step (2^103) past it rounds to an infinity (the
+    # distance of the type's lowest value from its highest is twice that)
+    want = np.where(want <= -(2.0 ** 128 - 2.0 ** 103), -np.inf, want)
     assert np.array_equal(np.isnan(got), np.isnan(want)), what
     assert np.array_equal(np.isneginf(got), np.isneginf(want)), what
     fine = np.isfinite(want)
@@ -258,6 +261,27 @@ def test_large_vocabularies_of_few_and_of_equal_logits(dtype, V):
     x[10, V - 1] = 30.0
     for K in (1, 20, 32):
         check(dtype, encode(dtype, x), rng.integers(0, V, (12, 2)), K)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("V", [100, 686, 2560, 2561, 40000, 150001])
+def test_masks_of_the_lowest_value(dtype, V):
+    """Forbidden tokens at the type's lowest finite value: fewer allowed ones than places, in every row a
+    different number; and rows of two values, of which the larger is rarer than the places are many."""
+    lowest = {BF16: -3.3895313892515355e38, F16: -65504.0, F32: -3.4028234663852886e38}[dtype]
+    rng = np.random.default_rng(11)
+    x = np.full((18, V), lowest)
+    for r in range(12):
+        some = rng.permutation(V)[:3 * r]
+        x[r, some] = rng.standard_normal(len(some)) * 2
+    x[12] = np.where(np.arange(V) % 2 == 0, lowest, -np.inf)
+    x[13, 7] = -lowest
+    x[14, rng.permutation(V)[:9]] = lowest / 2
+    x[15, rng.permutation(V)[:9]] = -lowest
+    x[16] = rng.standard_normal(V) * 2
+    x[17] = np.sort(rng.standard_normal(V))
+    for K in (1, 20, 32):
+        check(dtype, encode(dtype, x), rng.integers(0, V, (18, 2)), K)
 
 
 def test_the_workspace_has_to_be_there():
