@@ -21,6 +21,7 @@ struct LogprobsArgs {
     uint32_t R, V, G, K;
     uint32_t tile_cols, given_tile_cols, top_tile_cols;
     FastDiv div_rows;
+    FastDiv div_parts;               // pieces of sixteen tiles of a cell
     // how the scan is laid out
     uint32_t rows, bands;            // rows of all planes; tile rows of a plane
     uint32_t splits, cells_per_split, cells, cell_groups, group_tiles;
@@ -70,6 +71,17 @@ __device__ __forceinline__ float logit_of(u32x4 w, int i) {
     if constexpr (DT == IOMX_DT_F32) return as_f32(w[i]);
     else if constexpr (DT == IOMX_DT_BF16) return (i & 1) ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]);
     else { const f32x2 p = f16_pair(w[i >> 1]); return (i & 1) ? p.y : p.x; }
+}
+
+// A lane's value from another lane of its row of sixteen, by a move within the register file (a shuffle goes
+// through LDS); and the other half of the wave's.
+template <int CONTROL>
+__device__ __forceinline__ float lane_moved(float v) {
+    return as_f32(__builtin_amdgcn_update_dpp(as_u32(v), as_u32(v), CONTROL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float other_half(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(as_u32(v), as_u32(v), false, false);
+    return as_f32((threadIdx.x & 32u) ? both[0] : both[1]);
 }
 
 // GT: tiles of a group, which a wave loads at once
@@ -157,9 +169,9 @@ __global__ __launch_bounds__(256) void token_logprobs_scan_kernel(const Logprobs
         }
         if (a.cell_max) {
             // the lanes of a row: neighbours, and the other half of the wave where a load has two tiles
-            cell = fmaxf(cell, __shfl_xor(cell, 1));
-            if constexpr (kPerRow == 4) cell = fmaxf(cell, __shfl_xor(cell, 2));
-            else cell = fmaxf(cell, __shfl_xor(cell, 32));
+            cell = fmaxf(cell, lane_moved<0xB1>(cell));              // quad_perm 1, 0, 3, 2
+            if constexpr (kPerRow == 4) cell = fmaxf(cell, lane_moved<0x4E>(cell));      // 2, 3, 0, 1
+            else cell = fmaxf(cell, other_half(cell));
             if (there && part == 0 && lane_tile == 0) a.cell_max[((uint64_t)band * a.cells + c) * kTile + row] = cell;
         }
     }
@@ -205,10 +217,6 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 
 // Reductions over a wave by moves within the register file (a shuffle goes through LDS): rows of 16
 // lanes by four rotations, then the rows' results out of scalar registers.
-template <int CONTROL>
-__device__ __forceinline__ float lane_moved(float v) {
-    return as_f32(__builtin_amdgcn_update_dpp(as_u32(v), as_u32(v), CONTROL, 0xF, 0xF, false));
-}
 template <class Op>
 __device__ __forceinline__ float wave_reduce(float x, Op op) {
     x = op(x, lane_moved<0x121>(x));   // row_ror:1, 2, 4, 8
@@ -233,7 +241,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
     constexpr float inf = __builtin_inff();
     constexpr uint32_t kSlots = (SMALL ? kSmall : kMostCells) / 64, kMostListed = SMALL ? kMostCandidates : kMostChosen;
     const uint32_t all_cells = SMALL ? a.V : a.cells;
-    __shared__ uint64_t found[4][kMostCandidates];
+    __shared__ uint32_t found[4][kMostCandidates];       // columns
     __shared__ uint16_t chosen[4][kMostChosen];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t index = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);          // of the row
@@ -278,7 +286,188 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
     // a NaN or +inf left the sum a NaN
     const bool bad = !(sum > 0.0f);
     const float nan = as_f32(kQuietNanF32);
-    const double log_sum = log((double)sum), whole = (double)now + log_sum;
+    double log_sum, whole;
+    // (a hundred and more 64-bit instructions: where the loads of candidates are on their way)
+    auto form_log = [&]() __attribute__((always_inline)) {
+        log_sum = log((double)sum);
+        whole = (double)now + log_sum;
+    };
+    auto put = [&](uint32_t place, uint32_t id, float logit) __attribute__((always_inline)) {
+        const uint64_t at = (row_at * a.top_tile_cols + (place >> 4)) * kTileSlots + in_row + (place & 15u);
+        a.top_ids[plane[4] * a.top_plane + at] = bad ? -1 : (int32_t)id;
+        a.top_logprobs[plane[5] * a.top_plane + at] = bad ? nan : (float)((double)logit - whole);
+    };
+    // the K most likely tokens
+    auto pick = [&]() __attribute__((always_inline)) {
+        // A bound that at least K cells' maxima reach, so that at least K logits do, and not many more: from
+        // the row's maximum downwards in steps that double, then halving the last step.
+        auto reaching = [&](float bound) __attribute__((always_inline)) -> uint32_t {
+            uint32_t n = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i)
+                if (i * 64 < all_cells) n += __popcll(__ballot(cells[i] >= bound));
+            return n;
+        };
+        auto largest_below = [&](float limit) __attribute__((always_inline)) -> float {
+            float top = -inf;
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) top = fmaxf(top, cells[i] < limit ? cells[i] : -inf);
+            return wave_max(top);
+        };
+        uint32_t ties = ~0u;                           // cells of exactly the bound that are looked at
+        const float top = largest_below(inf);
+        float over = top, step = fmaxf(1.0f, fabsf(top) * 0.0078125f);   // `over`: fewer than K reach it, or it is the top
+        float bound;
+        uint32_t reached;
+        for (;;) {
+            bound = fmaxf(top - step, -3.4028234663852886e38f);          // that one: every finite logit
+            reached = reaching(bound);
+            if (reached >= a.K || bound == -3.4028234663852886e38f) break;
+            over = bound;
+            step *= 2.0f;
+        }
+        // (of few cells nearly all would be taken, and far more logits with them)
+        const uint32_t spare = (all_cells - a.K) / 4, enough = a.K + (spare < a.K / 2 ? spare : a.K / 2);
+        for (int halvings = 0; halvings < 12 && reached > enough; ++halvings) {
+            const float middle = bound * 0.5f + over * 0.5f;
+            const uint32_t n = reaching(middle);
+            if (n >= a.K) { bound = middle; reached = n; }
+            else over = middle;
+        }
+        if (reached > kMostListed) {
+            // (rows of equal logits) the K-th largest maximum itself: of the cells that have it, those
+            // with the lowest columns make up the K cells that hold the K most likely tokens
+            uint32_t larger = 0;
+            bound = top;
+            for (;;) {
+                uint32_t equal = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < kSlots; ++i) equal += __popcll(__ballot(cells[i] == bound));
+                if (larger + equal >= a.K) break;
+                larger += equal;
+                bound = largest_below(bound);
+            }
+            ties = a.K - larger;
+        }
+        // the logits that reach it
+        uint32_t count = 0, listed = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) {
+            if (i * 64 >= all_cells) break;
+            const uint64_t below = (1ull << lane) - 1, equal = __ballot(cells[i] == bound);
+            const bool take = cells[i] > bound || (cells[i] == bound && (uint32_t)__popcll(equal & below) < ties);
+            const uint64_t there = __ballot(take);
+            const uint32_t place = listed + __popcll(there & below);
+            if constexpr (SMALL) { if (take) found[wave][place] = i * 64 + lane; }
+            else if (take) chosen[wave][place] = (uint16_t)(i * 64 + lane);
+            listed += __popcll(there);
+            if (ties != ~0u) ties -= __popcll(equal) < ties ? __popcll(equal) : ties;
+        }
+        const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 8 or 16
+        if constexpr (SMALL) {
+            count = listed;
+            form_log();
+        } else {
+            __builtin_amdgcn_wave_barrier();       // a wave's LDS operations are in order
+            // A lane takes four columns of a tile; a wave, sixteen tiles: a part of one cell, or two or four
+            // cells.  The loads of four such pieces are on their way together (with eight a step of 16 rows takes
+            // 0.7 us longer, 2047 rows 0.7 us less).  Few logits reach the bound,
+            // so a lane only notes which of its own do, a bit each, and the columns are listed from the bits.
+            constexpr uint32_t kAhead = 4;
+            const uint32_t parts = (per_cell + 15) / 16, shift = per_cell < 16 ? per_cell == 4 ? 2 : 1 : 0;   // 2^shift cells
+            const uint32_t pieces = ((listed + (1u << shift) - 1) >> shift) * parts;
+            const uint32_t lane_cell = (lane >> 2) >> (4 - shift), lane_tile = (lane >> 2) - (lane_cell << (4 - shift));
+            // first of a lane's four columns of piece p, from a.V on if it has none
+            auto columns_of = [&](uint32_t p) __attribute__((always_inline)) -> uint32_t {
+                const uint32_t q = divided(p, parts, a.div_parts), entry = (q << shift) + lane_cell;
+                const uint32_t tile_in_cell = (p - q * parts) * 16 + lane_tile;
+                const uint32_t tile = (entry < listed ? chosen[wave][entry] : 0u) * per_cell + tile_in_cell;
+                return p < pieces && entry < listed && tile_in_cell < per_cell ? tile * kTile + (lane & 3u) * 4 : ~0u;
+            };
+            uint32_t p0 = 0;
+            do {
+                u32x4 x[kAhead];
+                uint32_t first[kAhead];
+#pragma unroll
+                for (uint32_t n = 0; n < kAhead; ++n) {
+                    first[n] = columns_of(p0 + n);
+                    // a tile's padding columns are read with it, and not looked at
+                    const uint8_t* at = row + ((uint64_t)(first[n] < a.V ? first[n] >> 4 : 0u) * kTileSlots + (lane & 3u) * 4) * kSize;
+                    if constexpr (DT == IOMX_DT_F32) x[n] = *reinterpret_cast<const u32x4*>(at);
+                    else {
+                        const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+                        x[n] = u32x4{w.x, w.y, 0, 0};
+                    }
+                }
+                if (p0 == 0) form_log();
+                uint32_t hits = 0;
+#pragma unroll
+                for (uint32_t n = 0; n < kAhead; ++n)
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j)
+                        hits |= (logit_of<DT>(x[n], j) >= bound && first[n] < a.V && first[n] + j < a.V ? 1u : 0u) << (4 * n + j);
+                for (uint64_t there; (there = __ballot(hits != 0)) != 0;) {
+                    const uint32_t bit = (uint32_t)__ffs(hits) - 1u, place = count + __popcll(there & ((1ull << lane) - 1));
+                    if (hits && place < kMostCandidates) found[wave][place] = columns_of(p0 + (bit >> 2)) + (bit & 3u);
+                    hits &= hits - 1;
+                    count += __popcll(there);
+                }
+                p0 += kAhead;
+            } while (p0 < pieces && count <= kMostCandidates);
+        }
+        if (SMALL || count <= kMostCandidates) {
+            __builtin_amdgcn_wave_barrier();
+            auto key_of = [&](uint32_t i) __attribute__((always_inline)) -> uint64_t {
+                if (i >= count) return 0;
+                const uint32_t id = found[wave][i];
+                return top_key(logit_at<DT>(row, id), id);
+            };
+            const uint64_t one = key_of(lane), two = key_of(lane + 64);
+            uint32_t before_one = 0, before_two = 0;
+            for (uint32_t i = 0; i < count; ++i) {
+                const uint64_t from = i < 64 ? one : two;
+                const uint64_t key = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(from >> 32), i & 63u) << 32
+                                   | (uint32_t)__builtin_amdgcn_readlane((uint32_t)from, i & 63u);
+                before_one += key > one;
+                before_two += key > two;
+            }
+            if (lane < count && before_one < a.K) put(before_one, key_id(one), key_value(one));
+            if (lane + 64 < count && before_two < a.K) put(before_two, key_id(two), key_value(two));
+            // too few finite logits: the first of the others follow
+            uint32_t place = count;
+            for (uint32_t c0 = 0; place < a.K && c0 < a.V; c0 += 64) {
+                const bool masked = c0 + lane < a.V && logit_at<DT>(row, c0 + lane) == -inf;
+                const uint64_t there = __ballot(masked);
+                const uint32_t mine = place + __popcll(there & ((1ull << lane) - 1));
+                if (masked && mine < a.K) put(mine, c0 + lane, -inf);
+                place += __popcll(there);
+            }
+            return;
+        }
+        // many equal logits at the bound: a pass over the chosen cells for each place
+        uint64_t last = ~0ull;
+        for (uint32_t place = 0; place < a.K; ++place) {
+            uint64_t best = 0;
+            for (uint32_t n = 0; n < listed; ++n) {
+                const uint32_t from = chosen[wave][n] * per_cell * kTile;
+                const uint32_t to = from + per_cell * kTile < a.V ? from + per_cell * kTile : a.V;
+                for (uint32_t c = from + lane; c < to; c += 64) {
+                    const uint64_t key = top_key(logit_at<DT>(row, c), c);
+                    best = key < last && key > best ? key : best;
+                }
+            }
+#pragma unroll
+            for (int off = 1; off < 64; off *= 2) {
+                const uint64_t other = __shfl_xor((unsigned long long)best, off);
+                best = other > best ? other : best;
+            }
+            last = best;
+            if (lane == 0) put(place, key_id(best), key_value(best));
+        }
+    };
+    if (a.top_ids && !bad) pick();
+    else form_log();
+    if (a.top_ids && bad && lane < a.K) put(lane, 0, 0.0f);
     for (uint32_t g = lane; g < a.G; g += 64) {
         if (g >= 64) {
             given = (uint32_t)a.tokens[plane[1] * a.given_plane + given_at(g)];
@@ -289,172 +478,6 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
     }
     if (a.entropy && lane == 0)
         a.entropy[plane[3] * a.entropy_plane + row_at * kTileSlots + in_row] = bad ? nan : (float)(log_sum - (double)weighted / sum);
-    if (!a.top_ids) return;
-    auto put = [&](uint32_t place, uint32_t id, float logit) {
-        const uint64_t at = (row_at * a.top_tile_cols + (place >> 4)) * kTileSlots + in_row + (place & 15u);
-        a.top_ids[plane[4] * a.top_plane + at] = bad ? -1 : (int32_t)id;
-        a.top_logprobs[plane[5] * a.top_plane + at] = bad ? nan : (float)((double)logit - whole);
-    };
-    if (bad) {
-        if (lane < a.K) put(lane, 0, 0.0f);
-        return;
-    }
-    // A bound that at least K cells' maxima reach, so that at least K logits do, and not many more: from
-    // the row's maximum downwards in steps that double, then halving the last step.
-    auto reaching = [&](float bound) __attribute__((always_inline)) -> uint32_t {
-        uint32_t n = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i)
-            if (i * 64 < all_cells) n += __popcll(__ballot(cells[i] >= bound));
-        return n;
-    };
-    auto largest_below = [&](float limit) __attribute__((always_inline)) -> float {
-        float top = -inf;
-#pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i) top = fmaxf(top, cells[i] < limit ? cells[i] : -inf);
-        return wave_max(top);
-    };
-    uint32_t ties = ~0u;                           // cells of exactly the bound that are looked at
-    const float top = largest_below(inf);
-    float over = top, step = fmaxf(1.0f, fabsf(top) * 0.0078125f);   // `over`: fewer than K reach it, or it is the top
-    float bound;
-    uint32_t reached;
-    for (;;) {
-        bound = fmaxf(top - step, -3.4028234663852886e38f);          // that one: every finite logit
-        reached = reaching(bound);
-        if (reached >= a.K || bound == -3.4028234663852886e38f) break;
-        over = bound;
-        step *= 2.0f;
-    }
-    // (of few cells nearly all would be taken, and far more logits with them)
-    const uint32_t spare = (all_cells - a.K) / 4, enough = a.K + (spare < a.K / 2 ? spare : a.K / 2);
-    for (int halvings = 0; halvings < 12 && reached > enough; ++halvings) {
-        const float middle = bound * 0.5f + over * 0.5f;
-        const uint32_t n = reaching(middle);
-        if (n >= a.K) { bound = middle; reached = n; }
-        else over = middle;
-    }
-    if (reached > kMostListed) {
-        // (rows of equal logits) the K-th largest maximum itself: of the cells that have it, those
-        // with the lowest columns make up the K cells that hold the K most likely tokens
-        uint32_t larger = 0;
-        bound = top;
-        for (;;) {
-            uint32_t equal = 0;
-#pragma unroll
-            for (uint32_t i = 0; i < kSlots; ++i) equal += __popcll(__ballot(cells[i] == bound));
-            if (larger + equal >= a.K) break;
-            larger += equal;
-            bound = largest_below(bound);
-        }
-        ties = a.K - larger;
-    }
-    // the logits that reach it
-    uint32_t count = 0, listed = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kSlots; ++i) {
-        if (i * 64 >= all_cells) break;
-        const uint64_t below = (1ull << lane) - 1, equal = __ballot(cells[i] == bound);
-        const bool take = cells[i] > bound || (cells[i] == bound && (uint32_t)__popcll(equal & below) < ties);
-        const uint64_t there = __ballot(take);
-        const uint32_t place = listed + __popcll(there & below);
-        if constexpr (SMALL) { if (take) found[wave][place] = top_key(cells[i], i * 64 + lane); }
-        else if (take) chosen[wave][place] = (uint16_t)(i * 64 + lane);
-        listed += __popcll(there);
-        if (ties != ~0u) ties -= __popcll(equal) < ties ? __popcll(equal) : ties;
-    }
-    const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 8 or 16
-    if constexpr (SMALL) count = listed;
-    else {
-        __builtin_amdgcn_wave_barrier();       // a wave's LDS operations are in order
-        // A lane takes four columns of a tile; a wave, sixteen tiles: a part of one cell, or two or four
-        // cells.  The loads of four such pieces are on their way together (with sixteen the code no
-        // longer fits and a step of 16 rows takes 2 us longer).
-        constexpr uint32_t kAhead = 4;
-        const uint32_t parts = (per_cell + 15) / 16, together = per_cell < 16 ? 16 / per_cell : 1;
-        const uint32_t pieces = (listed + together - 1) / together * parts;
-        for (uint32_t p0 = 0; p0 < pieces && count <= kMostCandidates; p0 += kAhead) {
-            float x[kAhead][4];
-            uint32_t first[kAhead];
-#pragma unroll
-            for (uint32_t n = 0; n < kAhead; ++n) {
-                const uint32_t p = p0 + n;
-                const uint32_t entry = together > 1 ? p * together + (lane >> 2) / per_cell : p / parts;
-                const uint32_t tile_in_cell = together > 1 ? (lane >> 2) % per_cell : p % parts * 16 + (lane >> 2);
-                const uint32_t tile = (entry < listed ? chosen[wave][entry] : 0u) * per_cell + tile_in_cell;
-                first[n] = tile * kTile + (lane & 3u) * 4;
-                const bool in = p < pieces && entry < listed && tile_in_cell < per_cell && tile < a.tile_cols;
-                // a tile's padding columns are read with it, and not looked at
-                const uint8_t* at = row + ((uint64_t)(in ? tile : 0u) * kTileSlots + (lane & 3u) * 4) * kSize;
-                if constexpr (DT == IOMX_DT_F32) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(at);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[n][j] = as_f32(w[j]);
-                } else {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(at);
-                    const u32x4 wide = {w.x, w.y, 0, 0};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[n][j] = logit_of<DT>(wide, j);
-                }
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) x[n][j] = in && first[n] + j < a.V ? x[n][j] : -inf;
-            }
-#pragma unroll
-            for (uint32_t n = 0; n < kAhead; ++n)
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint64_t there = __ballot(x[n][j] >= bound);
-                    if (!there) continue;
-                    const uint32_t place = count + __popcll(there & ((1ull << lane) - 1));
-                    if (x[n][j] >= bound && place < kMostCandidates) found[wave][place] = top_key(x[n][j], first[n] + j);
-                    count += __popcll(there);
-                }
-        }
-    }
-    if (SMALL || count <= kMostCandidates) {
-        __builtin_amdgcn_wave_barrier();
-        const uint64_t one = lane < count ? found[wave][lane] : 0, two = lane + 64 < count ? found[wave][lane + 64] : 0;
-        uint32_t before_one = 0, before_two = 0;
-        for (uint32_t i = 0; i < count; ++i) {
-            const uint64_t from = i < 64 ? one : two;
-            const uint64_t key = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(from >> 32), i & 63u) << 32
-                               | (uint32_t)__builtin_amdgcn_readlane((uint32_t)from, i & 63u);
-            before_one += key > one;
-            before_two += key > two;
-        }
-        if (lane < count && before_one < a.K) put(before_one, key_id(one), key_value(one));
-        if (lane + 64 < count && before_two < a.K) put(before_two, key_id(two), key_value(two));
-        // too few finite logits: the first of the others follow
-        uint32_t place = count;
-        for (uint32_t c0 = 0; place < a.K && c0 < a.V; c0 += 64) {
-            const bool masked = c0 + lane < a.V && logit_at<DT>(row, c0 + lane) == -inf;
-            const uint64_t there = __ballot(masked);
-            const uint32_t mine = place + __popcll(there & ((1ull << lane) - 1));
-            if (masked && mine < a.K) put(mine, c0 + lane, -inf);
-            place += __popcll(there);
-        }
-        return;
-    }
-    // many equal logits at the bound: a pass over the chosen cells for each place
-    uint64_t last = ~0ull;
-    for (uint32_t place = 0; place < a.K; ++place) {
-        uint64_t best = 0;
-        for (uint32_t n = 0; n < listed; ++n) {
-            const uint32_t from = chosen[wave][n] * per_cell * kTile;
-            const uint32_t to = from + per_cell * kTile < a.V ? from + per_cell * kTile : a.V;
-            for (uint32_t c = from + lane; c < to; c += 64) {
-                const uint64_t key = top_key(logit_at<DT>(row, c), c);
-                best = key < last && key > best ? key : best;
-            }
-        }
-#pragma unroll
-        for (int off = 1; off < 64; off *= 2) {
-            const uint64_t other = __shfl_xor((unsigned long long)best, off);
-            best = other > best ? other : best;
-        }
-        last = best;
-        if (lane == 0) put(place, key_id(best), key_value(best));
-    }
 }
 
 namespace {
@@ -542,6 +565,7 @@ int logprobs_layout(int dtype, LogprobsArgs* a, uint64_t* stats_floats, uint64_t
     const uint32_t groups = (a->tile_cols + a->group_tiles - 1) / a->group_tiles;
     a->cell_groups = (groups + kMostCells - 1) / kMostCells;
     a->cells = (groups + a->cell_groups - 1) / a->cell_groups;
+    a->div_parts = make_fast_div((a->cell_groups * a->group_tiles + 15) / 16);
     // six workgroups for each CU in all, a cell for each wave at the least
     const uint64_t bands = a->walk.planes * a->bands;
     uint64_t splits = bands >= 1536 ? 1 : (1536 + bands - 1) / bands;
