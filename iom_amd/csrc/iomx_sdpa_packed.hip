@@ -402,6 +402,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     using Shape = PackedShape<DT, KS, W>;
     using Acc = typename Shape::Acc;
     constexpr int WK = 4 / WQ, DTL = 2 * KS, QUADS = Shape::kQuads;
+    constexpr bool kScarce = packed_waves(KS, WQ, NT) == 3 || (KS == 8 && W == 32);     // registers are
     constexpr uint32_t BM = W * QT * WQ, kStage = NT * KS * 1024;
     // Two stages of K and V, variables of their own and named where they are used: the compiler then
     // knows that a read of one need not wait for the loader's writes to the other.
@@ -461,7 +462,11 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     for (int q = 0; q < QT; ++q) row_of[q] = divided(m_wave + W * q + column, a.group, a.div_group);
     const bool idle = m_wave >= m_end;
     const uint32_t row_tiles = a.d_tiles * kTile16;
-    const bool odd = a.d_tiles < (uint32_t)DTL;
+    // Feature tiles that a token tile's stage has room for and that there are none of (the last one; of
+    // heads above 128 up to three) are not loaded: those of K meet zeros of Q and have to be
+    // finite, those of V are in no output.
+    constexpr uint32_t kSpare = KS > 4 ? 3 : 1;
+    const uint32_t spare = DTL - a.d_tiles;
 
     u32x4 qf[QT][Shape::kSteps];
 #pragma unroll
@@ -476,13 +481,15 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
             if (m < m_end && tile < a.d_tiles) qf[q][c] = *reinterpret_cast<const u32x4*>(qr + tile * kTile16);
         }
     }
-    // with an odd number of feature tiles the last one of a token tile's stage is not loaded: it
-    // meets zeros of Q and has to be finite
-    if (odd) {
-        for (uint32_t i = threadIdx.x; i < WK * NT * 32; i += 256) {
-            const uint32_t at = (i >> 5) * (KS * 1024) + (DTL - 1) * kTile16 + (i & 31u) * 16;
+    if (spare) {
+        for (uint32_t i = threadIdx.x; i < WK * NT * kSpare * 32; i += 256) {
+            const uint32_t tile = DTL - kSpare + (i >> 5) % kSpare;
+            if (tile < a.d_tiles) continue;
+            const uint32_t at = i / (kSpare * 32) * (KS * 1024) + tile * kTile16 + (i & 31u) * 16;
             *reinterpret_cast<u32x4*>(&k_even[0][0] + at) = u32x4{0, 0, 0, 0};
             *reinterpret_cast<u32x4*>(&k_odd[0][0] + at) = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(&v_even[0][0] + at) = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(&v_odd[0][0] + at) = u32x4{0, 0, 0, 0};
         }
         __syncthreads();
     }
@@ -507,7 +514,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
         // (where registers are scarce, not to be known as the same lane every time: the addresses formed
         // from it would be kept in registers throughout the loop)
         uint32_t own_lane = lane;
-        if constexpr (packed_waves(KS, WQ, NT) == 3) asm volatile("" : "+v"(own_lane));
+        if constexpr (kScarce) asm volatile("" : "+v"(own_lane));
 #pragma unroll
         for (int n = 0; n < NT / WQ; ++n) {
             const uint32_t at = member + n * WQ;
@@ -527,7 +534,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
             }
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
-                if (c == KS - 1 && odd && lane >= 32) break;
+                if (2 * c + 2 > DTL - (int)kSpare && spare && 2 * c + (lane >> 5) >= a.d_tiles) break;
                 __builtin_amdgcn_global_load_lds((gptr_t)(kt + c * 1024 + Shape::k_source(own_lane, at) * 16), (lptr_t)(ks + at * (KS * 1024) + c * 1024), 16, 0, 0);
                 __builtin_amdgcn_global_load_lds((gptr_t)(vt + c * 1024 + Shape::v_source(own_lane) * 16), (lptr_t)(vs + at * (KS * 1024) + c * 1024), 16, 0, 0);
             }
@@ -678,7 +685,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
                             if (a.tree.base) {
                                 if (m_wave + W * q + column < m_end) {
                                     uint32_t row = seq.start + row_of[q];
-                                    if constexpr (packed_waves(KS, WQ, NT) == 3) asm volatile("" : "+v"(row));   // (as in fetch)
+                                    if constexpr (kScarce) asm volatile("" : "+v"(row));   // (as in fetch)
                                     const int32_t w = j >> 5;              // -1 for the rows before the first
                                     const uint32_t lo = w >= 0 && w < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w) : 0u;
                                     const uint32_t hi = w + 1 < (int32_t)a.tree.cols ? (uint32_t)a.tree.at(row, w + 1) : 0u;
@@ -1071,11 +1078,13 @@ struct PackedPlan {
 
 int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
     *p = {};
-    p->mfma = path != 1 && a.D % kTile == 0 && a.D <= 128 && (!a.table.base || a.page_rows % kTile == 0);
+    p->mfma = path != 1 && a.D % kTile == 0 && (!a.table.base || a.page_rows % kTile == 0);
     if (!p->mfma) return IOMX_OK;
     const uint64_t m = (uint64_t)a.max_rows * a.group;       // rows of the longest sequence, per KV head
-    p->columns = m <= 16 ? 16 : 32;
-    p->row_waves = m <= 32 ? 1 : m <= 64 ? 2 : 4;
+    // (four teams' stages of heads above 128 do not fit the LDS of a CU)
+    const bool wide = a.D > 128;
+    p->columns = m <= (wide ? 32 : 16) ? 16 : 32;
+    p->row_waves = m <= 32 ? wide ? 2 : 1 : m <= 64 ? 2 : 4;
     p->block_rows = (uint32_t)(p->columns * p->row_waves);
     p->row_blocks = (uint32_t)((m + p->block_rows - 1) / p->block_rows);
     p->groups = (uint64_t)a.sequences * a.Hkv * p->row_blocks;
@@ -1086,7 +1095,7 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
     const uint64_t capacity = (uint64_t)a.table.cols * a.page_rows + a.max_rows;
     if (p->groups < (p->block_rows <= 32 ? kPackedGroups : kPackedGroups / 2) && capacity > 2 * kPackedLeastTokens) {
         // (few rows of wide heads: a workgroup's stages fill the LDS of a CU)
-        const uint32_t groups = p->row_waves == 1 && a.D > 64 ? kPackedGroups / 2 : kPackedGroups;
+        const uint32_t groups = wide || (p->row_waves == 1 && a.D > 64) ? kPackedGroups / 2 : kPackedGroups;
         p->places = (groups + (uint32_t)a.Hkv - 1) / (uint32_t)a.Hkv;
         // (the row blocks there may be and one more piece for each of packed_room's at the most)
         const uint64_t most = p->block_rows <= 32 ? 2 * p->groups / a.Hkv : 0;
@@ -1109,7 +1118,11 @@ void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, hipStream_t st)
 
 template <int DT, int KS>
 void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, hipStream_t st) {
-    if (p.columns == 16) launch_packed<DT, KS, 16, 1, 2>(a, p, st);
+    if constexpr (KS > 4) {
+        if (p.columns == 16) launch_packed<DT, KS, 16, 2, 2>(a, p, st);
+        else if (p.row_waves == 2) launch_packed<DT, KS, 32, 2, 2>(a, p, st);
+        else launch_packed<DT, KS, 32, 4, 4>(a, p, st);
+    } else if (p.columns == 16) launch_packed<DT, KS, 16, 1, 2>(a, p, st);
     else if (p.row_waves == 1) launch_packed<DT, KS, 32, 1, 2>(a, p, st);
     else if (p.row_waves == 2) launch_packed<DT, KS, 32, 2, 2>(a, p, st);
     else launch_packed<DT, KS, 32, 4, 4>(a, p, st);
@@ -1121,7 +1134,9 @@ void launch_packed(const SdpaPackedArgs& a, const PackedPlan& p, hipStream_t st)
         case 1: launch_packed<DT, 1>(a, p, st); break;
         case 2: launch_packed<DT, 2>(a, p, st); break;
         case 3: launch_packed<DT, 3>(a, p, st); break;
-        default: launch_packed<DT, 4>(a, p, st); break;
+        case 4: launch_packed<DT, 4>(a, p, st); break;
+        case 5: case 6: launch_packed<DT, 6>(a, p, st); break;
+        default: launch_packed<DT, 8>(a, p, st); break;
     }
 }
 

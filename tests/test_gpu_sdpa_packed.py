@@ -358,6 +358,17 @@ def test_every_division_of_the_work(dtype, D, rows, long, tree):
     case.check(case.run())
 
 
+@pytest.mark.parametrize("dtype,D", [(BF16, 144), (F16, 160), (BF16, 192), (F16, 208), (F16, 240), (BF16, 256)])
+@pytest.mark.parametrize("rows", [4, 8, 16, 32, 33, 70])
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("tree", [False, True])
+def test_every_division_of_the_work_of_wide_heads(dtype, D, rows, long, tree):
+    ctx = [2300, 0, 700, 1537] if long else [200, 0, 31, 64]
+    case = Attention(54, dtype, (4, 1), D, 64, [rows, 1, rows - 1, rows // 2], ctx, tree=tree, tail=1)
+    case.check(case.run())
+    assert iomx.last_launch().kernel.decode() != "sdpa_packed_rows"
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_more_sequences_than_lanes(dtype):
     """The shares of 150 sequences, most of them short or without rows."""
