@@ -36,13 +36,16 @@ struct LogprobsArgs {
 // tile row).  It keeps the row's maximum M, sum e^d and sum d e^d with d = x - M (a difference, not a
 // product with log2 e taken from another: logits near the ends of the range stay finite), 64,
 // 32 or 16 logits at a time with the maximum moved before each, and the maximum of every cell (a group
-// of 64 to 256 columns, or a few groups) goes to the workspace.  2047 rows of 128256 BF16: 103 us, 5.1
+// of 64 to 256 columns, or a few groups) goes to the workspace.  2047 rows of 128256 BF16: 102 us, 5.1
 // TB/s, what a read of as many bytes reaches; the vector units are busy for two thirds of it.
 //
 // token_logprobs_finish, one wave per row, joins the sums and picks the most likely tokens without
 // another pass: a value that K cells' maxima reach is reached by K logits, so only the cells that
 // reach it are read again, and in them the logits that reach it are few; each counts those before it
-// (larger, or equal with a lower id), which is its place.
+// (larger, or equal with a lower id), which is its place.  Bound by that gather: 28 us for 2047 rows and
+// their 20 most likely (112 MB in lines of 128 bytes, of which a row has a quarter), of which 2 us look
+// for the bound; twice as many cells of half the size save 4 us here and cost the scan 10 us.  Few rows wait
+// for three reads one after the other: 8.5 us for 16.
 // ---------------------------------------------------------------------------
 
 constexpr uint32_t kMostCells = 512;          // of a row: eight per lane

@@ -61,7 +61,11 @@ __device__ __forceinline__ PackedSequence packed_sequence(const SdpaPackedArgs& 
 }
 
 // One wave = one row of one head: 64 tokens at a time, a lane forms the score of one token, then
-// the lanes take the features.  Running maximum and sum; everything in F32.
+// the lanes take the features, four tokens' values on their way together (with eight, 15.4 ms instead
+// of 13.1 for the prompts below).  Running maximum and sum; everything in F32.  For head sizes of no
+// whole tiles, pages of another size than whole tiles, and as a check of the matrix cores' kernel: every row reads
+// K and V for itself, bound by the latency of these reads and by F32 arithmetic (24 prompts of up to 1201
+// rows, 32 / 4 heads of 64: 13 ms, 5 TFLOP/s, where the matrix cores take 0.17 ms).
 template <int DT>
 __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedArgs a) {
     __shared__ float q_rows[4][kMaxPackedWidth];
@@ -75,18 +79,23 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
     const uint8_t* vb = a.v + hkv * a.v_head;
     const int32_t* pages = a.table.base ? a.table.row(s) : nullptr;
     const uint32_t row_tiles = a.d_tiles * kTile16;
-    // address of a token's row (null: absent)
-    auto token_row = [&](const uint8_t* own, const uint8_t* pool, uint64_t page_bytes, uint64_t head_bytes,
-                         uint32_t x) -> const uint8_t* {
+    // addresses of a token's rows; false: absent
+    auto token_rows = [&](uint32_t x, const uint8_t** kr, const uint8_t** vr) -> bool {
         if (x >= seq.cached) {
             const uint32_t t = seq.start + (x - seq.cached);
-            return own + (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32;
+            const uint64_t at = (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32;
+            *kr = kb + at;
+            *vr = vb + at;
+            return true;
         }
         const uint32_t slot = divided(x, a.page_rows, a.div_page_rows);
         const uint32_t page = (uint32_t)pages[(uint64_t)(slot >> 4) * kTileSlots + (slot & 15u)];
-        if (page >= a.pages) return nullptr;
+        if (page >= a.pages) return false;
         const uint32_t r = x - slot * a.page_rows;
-        return pool + page * page_bytes + hkv * head_bytes + (uint64_t)(r >> 4) * row_tiles + (r & 15u) * 32;
+        const uint64_t at = (uint64_t)(r >> 4) * row_tiles + (r & 15u) * 32;
+        *kr = a.k_pages + page * a.k_page + hkv * a.k_page_head + at;
+        *vr = a.v_pages + page * a.v_page + hkv * a.v_page_head + at;
+        return true;
     };
     auto element = [&](const uint8_t* row, uint32_t d) {
         return wide16<DT>(*reinterpret_cast<const uint16_t*>(row + (d >> 4) * kTile16 + (d & 15u) * 2));
@@ -106,12 +115,20 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
                 const uint32_t j = x - seq.cached;
                 seen = ((uint32_t)a.tree.at(t, j >> 5) >> (j & 31u)) & 1u;
             }
-            const uint8_t* kr = seen ? token_row(kb, a.k_pages, a.k_page, a.k_page_head, x) : nullptr;
-            seen = kr != nullptr;
+            // (a token that is not seen has the address of one that is there, the row's own)
+            const uint8_t *kr = nullptr, *vr = vb + (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32;
+            seen = seen && token_rows(x, &kr, &vr);
             float score = -inf;
             if (seen) {
                 score = 0.0f;
-                for (uint32_t d = 0; d < a.D; ++d) score = __builtin_fmaf(q_rows[wave][d], element(kr, d), score);
+                uint32_t d = 0;
+                for (; d + 8 <= a.D; d += 8) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(kr + (d >> 4) * kTile16 + (d & 15u) * 2);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        score = __builtin_fmaf(q_rows[wave][d + j], wide16<DT>(w[j >> 1] >> (16 * (j & 1)) & 0xFFFFu), score);
+                }
+                for (; d < a.D; ++d) score = __builtin_fmaf(q_rows[wave][d], element(kr, d), score);
             }
             float top = score;
             for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
@@ -126,14 +143,24 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[c] *= keep;
             const uint64_t any = __ballot(seen);
-            for (uint32_t y = 0; y < 64; ++y) {
-                if (!((any >> y) & 1u)) continue;
-                const float py = __shfl(p, y);
-                const uint8_t* vr = token_row(vb, a.v_pages, a.v_page, a.v_page_head, x0 + y);
+            const uint64_t at = reinterpret_cast<uint64_t>(vr);
+            for (uint32_t y0 = 0; y0 < 64; y0 += 4) {
+                if (!((any >> y0) & 15u)) continue;
+                float value[4][4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const uint32_t d = lane + 64 * c;
-                    if (d < a.D) acc[c] = __builtin_fmaf(py, element(vr, d), acc[c]);
+                for (int y = 0; y < 4; ++y) {
+                    const uint8_t* of = reinterpret_cast<const uint8_t*>(
+                            (uint64_t)__builtin_amdgcn_readlane((uint32_t)(at >> 32), y0 + y) << 32
+                            | (uint32_t)__builtin_amdgcn_readlane((uint32_t)at, y0 + y));
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) value[y][c] = lane + 64 * c < a.D ? element(of, lane + 64 * c) : 0.0f;
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    if (!((any >> (y0 + y)) & 1u)) continue;
+                    const float py = as_f32(__builtin_amdgcn_readlane(as_u32(p), y0 + y));
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(py, value[y][c], acc[c]);
                 }
             }
         }
@@ -169,6 +196,11 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // the second product (its error is half a step of each probability, as much as a value's own); the
 // sum is taken of the unrounded ones.  F16 lifts p by 2^kLift so that small probabilities keep their
 // bits: they are at most 2^(kLift + kSlack), and subnormal below 2^-22 of the largest.
+//
+// Long prompts are bound by the matrix cores and the exponentials beside them (8191 rows, 32 / 8 heads
+// of 128 BF16: 573 us, 960 TFLOP/s of 1212 that a large product reaches; rows of 17 to 61 per sequence
+// and shorter prompts wait more: 24 prompts of up to 1201 rows of 64 take 174 us, 390 TFLOP/s), single tokens by
+// memory (32 tokens over 700 to 15001 cached ones, 8 KV heads of 128: 194 us, 5.2 TB/s).
 //
 // Only blocks that a row does not see in full (the ends of the cached prefix, the diagonal, trees,
 // absent pages) form masks.  There V is cleared where no row may see it, and a value left that is
@@ -938,8 +970,9 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     }
 }
 
-// A wave joins the rows of a sequence and KV head whose tokens were shared out: a lane takes four
-// features of a row, and scales each part from its own reference.
+// Joins the rows of a sequence and KV head whose tokens were shared out: a lane takes four features of
+// a row, and scales each part from its own reference.  Bound by the chain of reads that finds the
+// shares and then the parts: 7 us for 32 tokens, 9.4 us for eight trees of up to 61 rows (32 / 8 heads of 128).
 template <int DT, uint32_t BM, uint32_t NT>
 __global__ __launch_bounds__(256) void sdpa_packed_join_kernel(const SdpaPackedArgs a) {
     const uint32_t chunks = a.D / 4;
