@@ -39,7 +39,7 @@ struct LogprobsArgs {
 // of 64 to 256 columns, or a few groups) goes to the workspace.  2047 rows of 128256 BF16: 102 us, 5.1
 // TB/s, what a read of as many bytes reaches; the vector units are busy for two thirds of it.
 //
-// token_logprobs_finish, one wave per row, joins the sums and picks the most likely tokens without
+// token_logprobs_finish, one wave per row (or four), joins the sums and picks the most likely tokens without
 // another pass: a value that K cells' maxima reach is reached by K logits, so only the cells that
 // reach it are read again, and in them the logits that reach it are few; each counts those before it
 // (larger, or equal with a lower id), which is its place.  Bound by that gather: 28 us for 2047 rows and
@@ -53,6 +53,7 @@ constexpr uint32_t kMostChosen = 256;         // cells that are read again
 // Logits of a row that a wave holds: up to here they are their own cells, since with no more cells than places
 // nearly every logit is above the bound (686 logits, their 20 most likely: 55 us by cells of 64, 20 us by logits).
 constexpr uint32_t kSmall = 2560;
+constexpr uint32_t kTeamRows = 512;           // up to here four waves may pick from a row
 constexpr uint32_t kMostCandidates = 128;     // of a row: two per lane
 
 // d as a factor of e^d: from -200 on down e^d is 0 in F32, and its product with d is, too
@@ -237,8 +238,9 @@ __device__ __forceinline__ float wave_sum(float x) {
     return wave_reduce(x, [](float a, float b) { return a + b; });
 }
 
-// SMALL: a vocabulary of at most kSmall tokens, whose logits are their own cells.
-template <int DT, bool SMALL>
+// SMALL: a vocabulary of at most kSmall tokens, whose logits are their own cells.  TEAM: waves of a row (1 or
+// 4), which all look for the bound and share out the cells that are read again.
+template <int DT, bool SMALL, uint32_t TEAM>
 __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const LogprobsArgs a) {
     constexpr int kSize = DT == IOMX_DT_F32 ? 4 : 2;
     constexpr float inf = __builtin_inff();
@@ -246,8 +248,9 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
     const uint32_t all_cells = SMALL ? a.V : a.cells;
     __shared__ uint32_t found[4][kMostCandidates];       // columns
     __shared__ uint16_t chosen[4][kMostChosen];
+    __shared__ uint32_t counts[4];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t index = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + wave);          // of the row
+    const uint32_t index = __builtin_amdgcn_readfirstlane(TEAM > 1 ? blockIdx.x : blockIdx.x * 4 + wave);   // of the row
     if (index >= a.rows) return;
     const uint32_t plane_index = divided(index, a.R, a.div_rows), r = index - plane_index * a.R;
     const uint32_t band = plane_index * a.bands + (r >> 4);
@@ -387,7 +390,8 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
                 const uint32_t tile = (entry < listed ? chosen[wave][entry] : 0u) * per_cell + tile_in_cell;
                 return p < pieces && entry < listed && tile_in_cell < per_cell ? tile * kTile + (lane & 3u) * 4 : ~0u;
             };
-            uint32_t p0 = 0;
+            const uint32_t p_first = TEAM > 1 ? wave * kAhead : 0;
+            uint32_t p0 = p_first;
             do {
                 u32x4 x[kAhead];
                 uint32_t first[kAhead];
@@ -402,7 +406,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
                         x[n] = u32x4{w.x, w.y, 0, 0};
                     }
                 }
-                if (p0 == 0) form_log();
+                if (p0 == p_first) form_log();
                 uint32_t hits = 0;
 #pragma unroll
                 for (uint32_t n = 0; n < kAhead; ++n)
@@ -415,14 +419,23 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
                     hits &= hits - 1;
                     count += __popcll(there);
                 }
-                p0 += kAhead;
+                p0 += TEAM * kAhead;
             } while (p0 < pieces && count <= kMostCandidates);
+            if constexpr (TEAM > 1) {
+                if (lane == 0) counts[wave] = count;
+                __syncthreads();
+                if (wave) return;
+                count = counts[0] + counts[1] + counts[2] + counts[3];
+            }
         }
         if (SMALL || count <= kMostCandidates) {
             __builtin_amdgcn_wave_barrier();
             auto key_of = [&](uint32_t i) __attribute__((always_inline)) -> uint64_t {
                 if (i >= count) return 0;
-                const uint32_t id = found[wave][i];
+                uint32_t from = wave;
+                if constexpr (TEAM > 1)
+                    for (from = 0; i >= counts[from]; ++from) i -= counts[from];
+                const uint32_t id = found[from][i];
                 return top_key(logit_at<DT>(row, id), id);
             };
             const uint64_t one = key_of(lane), two = key_of(lane + 64);
@@ -470,6 +483,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
     };
     if (a.top_ids && !bad) pick();
     else form_log();
+    if (TEAM > 1 && wave) return;
     if (a.top_ids && bad && lane < a.K) put(lane, 0, 0.0f);
     for (uint32_t g = lane; g < a.G; g += 64) {
         if (g >= 64) {
@@ -590,9 +604,15 @@ void launch_logprobs(const LogprobsArgs& a, hipStream_t st) {
     else if (a.group_tiles == 4) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, 4, false>), grid, dim3(256), 0, st, a);
     else if (a.entropy) hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, kWideGroup<DT>, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((token_logprobs_scan_kernel<DT, kWideGroup<DT>, false>), grid, dim3(256), 0, st, a);
+    // Four waves of a row where there are few rows, and more pieces of cells than a wave has on their way
+    // together: 16 rows of 128256, 20 most likely, 17.5 us and 22.6 with one wave; 333 rows of 50257 F32, 8
+    // most likely, 24.7 and 26.0; 1024 rows of 32000, 10 most likely, 28.0 and 26.1; 16 rows of 32000, 5 most
+    // likely (three pieces), 12.5 and 12.2.
+    const bool team = a.rows <= kTeamRows && a.K * a.cell_groups * a.group_tiles > 64;
     const dim3 rows((a.rows + 3) / 4);
-    if (a.V <= kSmall) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, true>), rows, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, false>), rows, dim3(256), 0, st, a);
+    if (a.V <= kSmall) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, true, 1>), rows, dim3(256), 0, st, a);
+    else if (team) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, false, 4>), dim3(a.rows), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, false, 1>), rows, dim3(256), 0, st, a);
     record_launch("token_logprobs", grid.x, 256, (uint64_t)a.rows * a.V);
 }
 

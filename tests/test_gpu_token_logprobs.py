@@ -284,6 +284,26 @@ def test_masks_of_the_lowest_value(dtype, V):
         check(dtype, encode(dtype, x), rng.integers(0, V, (18, 2)), K)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows", [512, 513])
+def test_few_and_many_rows(dtype, rows):
+    """The last number of rows from which several waves pick, and one more; ordinary rows, equal logits,
+    few finite ones, and more candidates than are held."""
+    V = 9001
+    rng = np.random.default_rng(12)
+    x = rng.standard_normal((rows, V)) * 2
+    for r in range(0, 60, 6):
+        x[r] = 0.25
+        x[r + 1, rng.permutation(V)[:40 * r + 3]] = 20.0
+        x[r + 2] = -np.inf
+        x[r + 2, rng.permutation(V)[:r + 1]] = rng.standard_normal(r + 1)
+        x[r + 3] = -65504.0
+        x[r + 3, rng.permutation(V)[:r]] = 1.5
+        x[r + 4, 17 * r:17 * r + 300] = 20.0
+        x[r + 5] = np.sort(x[r + 5])
+    check(dtype, encode(dtype, x), rng.integers(0, V, (rows, 1)), 32)
+
+
 def test_the_workspace_has_to_be_there():
     t = {"logits": iomx.DeviceTensor(BF16, (3, 500)), "entropy": iomx.DeviceTensor(F32, (3, 1), fill=0x5A)}
     views = {n: x.view() for n, x in t.items()}
