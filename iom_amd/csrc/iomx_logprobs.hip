@@ -50,9 +50,10 @@ struct LogprobsArgs {
 
 constexpr uint32_t kMostCells = 512;          // of a row: eight per lane
 constexpr uint32_t kMostChosen = 256;         // cells that are read again
-// Logits of a row that a wave holds: up to here they are their own cells, since with no more cells than places
-// nearly every logit is above the bound (686 logits, their 20 most likely: 55 us by cells of 64, 20 us by logits).
-constexpr uint32_t kSmall = 2560;
+// Where a row has hardly more cells than places, nearly every logit is above the bound; its logits are then
+// their own cells, and a wave holds them all, sixteen or 38 per lane (5 rows of 686 logits, their 20 most
+// likely: 55 us by cells of 64, 14 us by logits; 2000 logits: 13 us by cells, 24 us by logits).
+constexpr uint32_t kFewSlots = 16, kMoreSlots = 38;
 constexpr uint32_t kTeamRows = 512;           // up to here four waves may pick from a row
 constexpr uint32_t kMostCandidates = 128;     // of a row: two per lane
 
@@ -238,14 +239,14 @@ __device__ __forceinline__ float wave_sum(float x) {
     return wave_reduce(x, [](float a, float b) { return a + b; });
 }
 
-// SMALL: a vocabulary of at most kSmall tokens, whose logits are their own cells.  TEAM: waves of a row (1 or
+// OWN: slots of a lane for logits that are their own cells; 0: cells of the scan.  TEAM: waves of a row (1 or
 // 4), which all look for the bound and share out the cells that are read again.
-template <int DT, bool SMALL, uint32_t TEAM>
+template <int DT, uint32_t OWN, uint32_t TEAM>
 __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const LogprobsArgs a) {
     constexpr int kSize = DT == IOMX_DT_F32 ? 4 : 2;
     constexpr float inf = __builtin_inff();
-    constexpr uint32_t kSlots = (SMALL ? kSmall : kMostCells) / 64, kMostListed = SMALL ? kMostCandidates : kMostChosen;
-    const uint32_t all_cells = SMALL ? a.V : a.cells;
+    constexpr uint32_t kSlots = OWN ? OWN : kMostCells / 64, kMostListed = OWN ? kMostCandidates : kMostChosen;
+    const uint32_t all_cells = OWN ? a.V : a.cells;
     __shared__ uint32_t found[4][kMostCandidates];       // columns
     __shared__ uint16_t chosen[4][kMostChosen];
     __shared__ uint32_t counts[4];
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i) {
             const uint32_t c = i * 64 + lane;
-            if constexpr (SMALL) cells[i] = c < a.V ? logit_at<DT>(row, c) : -inf;
+            if constexpr (OWN != 0) cells[i] = c < a.V ? logit_at<DT>(row, c) : -inf;
             else cells[i] = c < a.cells ? maxima[(uint64_t)c * kTile] : -inf;
         }
     }
@@ -364,13 +365,13 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
             const bool take = cells[i] > bound || (cells[i] == bound && (uint32_t)__popcll(equal & below) < ties);
             const uint64_t there = __ballot(take);
             const uint32_t place = listed + __popcll(there & below);
-            if constexpr (SMALL) { if (take) found[wave][place] = i * 64 + lane; }
+            if constexpr (OWN != 0) { if (take) found[wave][place] = i * 64 + lane; }
             else if (take) chosen[wave][place] = (uint16_t)(i * 64 + lane);
             listed += __popcll(there);
             if (ties != ~0u) ties -= __popcll(equal) < ties ? __popcll(equal) : ties;
         }
         const uint32_t per_cell = a.cell_groups * a.group_tiles;                 // tiles: 4, or a multiple of 8 or 16
-        if constexpr (SMALL) {
+        if constexpr (OWN != 0) {
             count = listed;
             form_log();
         } else {
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
                 count = counts[0] + counts[1] + counts[2] + counts[3];
             }
         }
-        if (SMALL || count <= kMostCandidates) {
+        if (OWN || count <= kMostCandidates) {
             __builtin_amdgcn_wave_barrier();
             auto key_of = [&](uint32_t i) __attribute__((always_inline)) -> uint64_t {
                 if (i >= count) return 0;
@@ -571,6 +572,11 @@ int logprobs_request(int dtype, const iomx_view* logits, const iomx_view* tokens
 
 template <int DT> constexpr int kWideGroup = DT == IOMX_DT_F32 ? 16 : 8;
 
+// Fewer than a fifth more cells than places (the cells are of 64 columns then; with a tenth more, a row in
+// forty of 2241 logits has more than kMostCandidates above the bound of its 32 most likely).
+bool picks_from_logits(const LogprobsArgs& a) { return 5 * a.cells < 6 * a.K; }
+static_assert((6 * kMaxTop - 1) / 5 <= kMoreSlots, "a lane holds a slot of every such cell");
+
 // The scan's layout, and the floats of workspace it takes.
 int logprobs_layout(int dtype, LogprobsArgs* a, uint64_t* stats_floats, uint64_t* cell_floats) {
     // Groups of 64 columns for small vocabularies, so that even a row of few thousand logits has a
@@ -593,7 +599,7 @@ int logprobs_layout(int dtype, LogprobsArgs* a, uint64_t* stats_floats, uint64_t
     a->div_splits = make_fast_div(a->splits);
     if (bands * a->splits > 0x7FFFFFF0ull) return IOMX_ERR_OVERFLOW;
     *stats_floats = bands * a->splits * kTile * 4;
-    *cell_floats = a->top_ids && a->V > kSmall ? bands * a->cells * kTile : 0;
+    *cell_floats = a->top_ids && !picks_from_logits(*a) ? bands * a->cells * kTile : 0;
     return IOMX_OK;
 }
 
@@ -610,9 +616,10 @@ void launch_logprobs(const LogprobsArgs& a, hipStream_t st) {
     // likely (three pieces), 12.5 and 12.2.
     const bool team = a.rows <= kTeamRows && a.K * a.cell_groups * a.group_tiles > 64;
     const dim3 rows((a.rows + 3) / 4);
-    if (a.V <= kSmall) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, true, 1>), rows, dim3(256), 0, st, a);
-    else if (team) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, false, 4>), dim3(a.rows), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, false, 1>), rows, dim3(256), 0, st, a);
+    if (picks_from_logits(a) && a.V <= 64 * kFewSlots) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, kFewSlots, 1>), rows, dim3(256), 0, st, a);
+    else if (picks_from_logits(a)) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, kMoreSlots, 1>), rows, dim3(256), 0, st, a);
+    else if (team) hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, 0, 4>), dim3(a.rows), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((token_logprobs_finish_kernel<DT, 0, 1>), rows, dim3(256), 0, st, a);
     record_launch("token_logprobs", grid.x, 256, (uint64_t)a.rows * a.V);
 }
 

@@ -284,6 +284,22 @@ def test_masks_of_the_lowest_value(dtype, V):
         check(dtype, encode(dtype, x), rng.integers(0, V, (18, 2)), K)
 
 
+@pytest.mark.parametrize("dtype,V,K", [(BF16, 64, 1), (F16, 65, 1), (BF16, 1024, 20), (F32, 1025, 20), (F16, 1472, 20),
+                                       (BF16, 1473, 20), (BF16, 2432, 32), (F16, 2433, 32), (F32, 2433, 32)])
+def test_vocabularies_of_few_cells(dtype, V, K):
+    """On both sides of the sizes up to which a row's logits are picked from without cells."""
+    rng = np.random.default_rng(13)
+    x = rng.standard_normal((40, V)) * 2
+    x[3] = 0.25
+    x[4] = -np.inf
+    x[4, V // 2] = 1.0
+    x[5, :V // 2] = -np.inf
+    x[6] = np.sort(x[6])
+    x[7] = np.sort(x[7])[::-1]
+    x[8] = np.round(x[8])
+    check(dtype, encode(dtype, x), rng.integers(0, V, (40, 1)), K)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("rows", [512, 513])
 def test_few_and_many_rows(dtype, rows):
