@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // bits: they are at most 2^(kLift + kSlack), and subnormal below 2^-22 of the largest.
 //
 // Long prompts are bound by the matrix cores and the exponentials beside them (8191 rows, 32 / 8 heads
-// of 128 BF16: 573 us, 960 TFLOP/s of 1212 that a large product reaches; rows of 17 to 61 per sequence
+// of 128 BF16: 580 us, 950 TFLOP/s of 1212 that a large product reaches; rows of 17 to 61 per sequence
 // and shorter prompts wait more: 24 prompts of up to 1201 rows of 64 take 174 us, 390 TFLOP/s), single tokens by
 // memory (32 tokens over 700 to 15001 cached ones, 8 KV heads of 128: 194 us, 5.2 TB/s).
 //
@@ -652,6 +652,10 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     auto words = [&](uint32_t (&w)[2 * QUADS], int h) __attribute__((always_inline)) {
         return u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
     };
+    // (kYield: with two waves on a SIMD the one at its vector instructions goes first, since the other's matrix
+    // instructions run on by themselves: 581 us instead of 591 for the long prompt, 51.5 instead of 53 for trees; with
+    // three, short prompts take 176 us instead of 173.)
+    constexpr bool kYield = packed_waves(KS, WQ, NT) == 2;
     // A block that every row of the wave sees in full and whose scores are below the references, which
     // the wave's first block sets; false if they are not (nothing is changed then: any_pair takes the
     // block, and the sums, which only it scales, keep their registers here).
@@ -660,16 +664,22 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
         Acc sc[NT / 2][QT][Shape::kScores];
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) scores(ks + n * (2 * KS * 1024), sc[n]);
+        if constexpr (kYield) __builtin_amdgcn_s_setprio(1);
         float top[QT];
         largest(sc, top);
         if (!begun) {
 #pragma unroll
             for (int q = 0; q < QT; ++q) ref[q] = fmaxf(Shape::join(top[q]), kLowest);
-        } else if (beyond(top)) return false;
+        } else if (beyond(top)) {
+            if constexpr (kYield) __builtin_amdgcn_s_setprio(0);
+            return false;
+        }
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) {
             uint32_t pw[QT][2 * QUADS];
+            if constexpr (kYield) __builtin_amdgcn_s_setprio(1);
             probabilities(sc[n], pw);
+            if constexpr (kYield) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int h = 0; h < Shape::kHalves; ++h)
 #pragma unroll
