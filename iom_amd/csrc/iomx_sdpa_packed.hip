@@ -197,10 +197,10 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // sum is taken of the unrounded ones.  F16 lifts p by 2^kLift so that small probabilities keep their
 // bits: they are at most 2^(kLift + kSlack), and subnormal below 2^-22 of the largest.
 //
-// Long prompts are bound by the matrix cores and the exponentials beside them (8191 rows, 32 / 8 heads
-// of 128 BF16: 580 us, 950 TFLOP/s of 1212 that a large product reaches; rows of 17 to 61 per sequence
-// and shorter prompts wait more: 24 prompts of up to 1201 rows of 64 take 174 us, 390 TFLOP/s), single tokens by
-// memory (32 tokens over 700 to 15001 cached ones, 8 KV heads of 128: 194 us, 5.2 TB/s).
+// Long prompts are bound by the matrix and the vector units, busy for 0.43 and 0.44 of the cycles (8191 rows,
+// 32 / 8 heads of 128 BF16: 583 us, 940 TFLOP/s of 1212 that a large product reaches); shorter ones wait
+// more (24 prompts of up to 1201 rows of 64: 174 us, 390 TFLOP/s); single tokens are bound by memory (32
+// tokens over 700 to 15001 cached ones, 8 KV heads of 128: 194 us, 5.2 TB/s).
 //
 // Only blocks that a row does not see in full (the ends of the cached prefix, the diagonal, trees,
 // absent pages) form masks.  There V is cleared where no row may see it, and a value left that is
@@ -418,7 +418,7 @@ __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uin
 }
 
 // Waves per SIMD: as many workgroups as the stages leave room for in the LDS of a CU, up to two, or
-// three where the registers last (packed prompts of heads of 64 take 167 us with three and 207 us
+// three where the registers last (packed prompts of heads of 64 take 174 us with three and 207 us
 // with two).
 constexpr int packed_waves(int KS, int WQ, int NT) {
     const int fit = 160 * 1024 / (4 * (4 / WQ) * NT * KS * 1024 + 2048), most = KS <= 2 && WQ == 4 ? 3 : 2;
