@@ -412,7 +412,9 @@ int iomx_launch_softmax(const iomx_softmax_desc* desc, iomx_stream_t stream);
  * Page pools are [N, Hkv, P, D] views (a plane is one head of one page, so a pool may be
  * a slice of a larger tensor, and a dense cache [S, Hkv, C, D] is a pool of S pages of C
  * rows).  No value in these operands makes a kernel leave its tensors: starts are clamped
- * to [0, T], lengths to [0, M * P].
+ * to [0, T] (of the append, to [0, E]), lengths to [0, M * P].  A sequence whose start is
+ * past its end has no rows.  (Starts that fall may give a row to two sequences: the
+ * attention leaves either one's result there, the append writes the first one's.)
  */
 
 /*

@@ -123,21 +123,26 @@ struct AppendPackedArgs {
     FastDiv div_page_rows;
 };
 
-// The sequence of each of the sixteen entries e0 .. e0 + 15: the number of starts[1..] at or
-// below it.  The wave reads the starts 64 at a time, a word per lane, and counts with ballots:
-// one trip to memory for up to 64 sequences, where a search would be a chain of them.
+// The sequence of each of the sixteen entries e0 .. e0 + 15: the first one s with starts[s] <= e < starts[s + 1],
+// or `sequences`.  The wave reads the starts 64 at a time, a word per lane; a ballot tells which are at or below an
+// entry, and a sequence holds it whose start is and whose end is not: one trip to memory for up to 63
+// sequences, where a search would be a chain of them (and would need starts that do not fall).
 __device__ __forceinline__ uint32_t sequence_of(const IndexMatrix& starts, uint32_t sequences, uint32_t e0,
                                                 uint32_t which) {
     const uint32_t lane = threadIdx.x & 63u;
-    uint32_t found = 0;
-    for (uint32_t s0 = 0; s0 < sequences; s0 += 64) {
+    uint32_t found = sequences;
+    for (uint32_t s0 = 0; s0 < sequences; s0 += 63) {
         const uint32_t s = s0 + lane;
-        const int32_t bound = s < sequences ? starts.at(s + 1) : 0x7FFFFFFF;
+        const int32_t start = s <= sequences ? starts.at(s) : 0;
+        const uint32_t count = sequences - s0 < 63 ? sequences - s0 : 63;
+        uint64_t holds = 0;                      // bit: a sequence of these that holds the lane's entry
 #pragma unroll
         for (uint32_t i = 0; i < kTile; ++i) {
-            const uint32_t below = __popcll(__ballot(bound <= (int32_t)(e0 + i)));
-            if (which == i) found += below;
+            const uint64_t below = __ballot(start <= (int32_t)(e0 + i));
+            const uint64_t here = below & ~(below >> 1) & ((1ull << count) - 1);
+            holds = which == i ? here : holds;
         }
+        if (found == sequences && holds) found = s0 + (uint32_t)__ffsll((unsigned long long)holds) - 1u;
     }
     return found;
 }
@@ -156,13 +161,13 @@ __global__ __launch_bounds__(256) void cache_append_packed_kernel(const AppendPa
         const uint32_t e = band * kTile + which;
         const uint32_t s = sequence_of(a.starts, a.sequences, band * kTile, which);
         if (head >= a.heads || e >= a.entries || s >= a.sequences) continue;
-        const int32_t start = a.starts.at(s);
-        if (start < 0 || (uint32_t)start > e) continue;    // before the first sequence
+        const int32_t first = a.starts.at(s);
+        const uint32_t start = first < 0 ? 0u : (uint32_t)first;
         const uint32_t row = a.rows.base ? (uint32_t)a.rows.at(e) : e;
         if (row >= a.T) continue;
         const uint64_t capacity = (uint64_t)a.table.cols * a.page_rows;
         const int32_t length = a.lengths.at(s);
-        const uint64_t token = (uint64_t)(length < 0 ? 0 : length) + (e - (uint32_t)start);
+        const uint64_t token = (uint64_t)(length < 0 ? 0 : length) + (e - start);
         if (token >= capacity) continue;
         const uint32_t slot = divided((uint32_t)token, a.page_rows, a.div_page_rows);
         const uint32_t page = (uint32_t)a.table.at(s, slot);
