@@ -293,16 +293,17 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
     // a NaN or +inf left the sum a NaN
     const bool bad = !(sum > 0.0f);
     const float nan = as_f32(kQuietNanF32);
-    double log_sum, whole;
+    double log_sum;
     // (a hundred and more 64-bit instructions: where the loads of candidates are on their way)
-    auto form_log = [&]() __attribute__((always_inline)) {
-        log_sum = log((double)sum);
-        whole = (double)now + log_sum;
+    auto form_log = [&]() __attribute__((always_inline)) { log_sum = log((double)sum); };
+    // Of two logits of 1e38 the difference comes first: next to either of them the logarithm is lost in 64 bits too.
+    auto log_probability = [&](float logit) __attribute__((always_inline)) -> float {
+        return (float)((double)logit - (double)now - log_sum);
     };
     auto put = [&](uint32_t place, uint32_t id, float logit) __attribute__((always_inline)) {
         const uint64_t at = (row_at * a.top_tile_cols + (place >> 4)) * kTileSlots + in_row + (place & 15u);
         a.top_ids[plane[4] * a.top_plane + at] = bad ? -1 : (int32_t)id;
-        a.top_logprobs[plane[5] * a.top_plane + at] = bad ? nan : (float)((double)logit - whole);
+        a.top_logprobs[plane[5] * a.top_plane + at] = bad ? nan : log_probability(logit);
     };
     // the K most likely tokens
     auto pick = [&]() __attribute__((always_inline)) {
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(256) void token_logprobs_finish_kernel(const Logpro
             if (given < a.V) given_logit = logit_at<DT>(row, given);
         }
         a.logprobs[plane[2] * a.given_plane + given_at(g)] =
-                given >= a.V ? -inf : bad ? nan : (float)((double)given_logit - whole);
+                given >= a.V ? -inf : bad ? nan : log_probability(given_logit);
     }
     if (a.entropy && lane == 0)
         a.entropy[plane[3] * a.entropy_plane + row_at * kTileSlots + in_row] = bad ? nan : (float)(log_sum - (double)weighted / sum);
