@@ -1146,7 +1146,7 @@ int packed_plan(const SdpaPackedArgs& a, int path, PackedPlan* p) {
         p->stats_floats = (p->groups * p->block_rows * 2 + 63) / 64 * 64;
         p->parts_floats = p->groups * p->block_rows * a.D;
     }
-    if (p->groups > 0x7FFFFFF0ull) return IOMX_ERR_OVERFLOW;
+    if (p->groups > 0xFFFFFFull) return IOMX_ERR_OVERFLOW;     // a grid has fewer than 2^32 lanes
     return IOMX_OK;
 }
 
