@@ -60,16 +60,89 @@ __device__ __forceinline__ PackedSequence packed_sequence(const SdpaPackedArgs& 
     return p;
 }
 
-// One wave = one row of one head: 64 tokens at a time, a lane forms the score of one token, then
-// the lanes take the features, four tokens' values on their way together (with eight, 15.4 ms instead
-// of 13.1 for the prompts below).  Running maximum and sum; everything in F32.  For head sizes of no
-// whole tiles, pages of another size than whole tiles, and as a check of the matrix cores' kernel: every row reads
-// K and V for itself, bound by the latency of these reads and by F32 arithmetic (24 prompts of up to 1201
-// rows, 32 / 4 heads of 64: 13 ms, 5 TFLOP/s, where the matrix cores take 0.17 ms).
+template <int DT>
+__device__ __forceinline__ float packed_element(const uint8_t* row, uint32_t d) {
+    return wide16<DT>(*reinterpret_cast<const uint16_t*>(row + (d >> 4) * kTile16 + (d & 15u) * 2));
+}
+
+// What a wave found out about one row of one head over some tokens: the largest score, the sum of e^(score - most),
+// and the mean of the values by these weights, feature lane + 64 c in mean[c].
+struct PackedRow {
+    float most, sum, mean[4];
+};
+
+// One row: 64 tokens at a time, a lane forms the score of one token, then the lanes take the features, four
+// tokens' values on their way together (with eight, 15.4 ms instead of 13.1 for the prompts below).  Running maximum,
+// sum and mean (a sum of values may pass F32's range where their mean does not); everything in F32.
+// `q` is the row times 1 / sqrt(D), in LDS.  locate(n, &k_row, &v_row) says whether the row sees token n and where
+// it lies; `there` is the address of any row (read, and not used, for a token that is not seen).
+template <int DT, class Locate>
+__device__ __forceinline__ PackedRow packed_row(uint32_t D, const float* q, uint32_t tokens, const uint8_t* there,
+                                                const Locate& locate) {
+    const float inf = __builtin_inff();
+    const uint32_t lane = threadIdx.x & 63u;
+    PackedRow row = {-inf, 0.0f, {0, 0, 0, 0}};
+    for (uint32_t n0 = 0; n0 < tokens; n0 += 64) {
+        const uint8_t *kr = nullptr, *vr = there;
+        const bool seen = n0 + lane < tokens && locate(n0 + lane, &kr, &vr);
+        float score = -inf;
+        if (seen) {
+            score = 0.0f;
+            uint32_t d = 0;
+            for (; d + 8 <= D; d += 8) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(kr + (d >> 4) * kTile16 + (d & 15u) * 2);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    score = __builtin_fmaf(q[d + j], wide16<DT>(w[j >> 1] >> (16 * (j & 1)) & 0xFFFFu), score);
+            }
+            for (; d < D; ++d) score = __builtin_fmaf(q[d], packed_element<DT>(kr, d), score);
+        }
+        float top = score;
+        for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
+        const float m2 = fmaxf(row.most, top);
+        const float base = m2 == -inf ? 0.0f : m2;
+        const float p = seen ? expf(score - base) : 0.0f;   // a NaN score stays one
+        const float keep = row.most == -inf ? 0.0f : expf(row.most - base);
+        float part = p;
+        for (int off = 1; off < 64; off *= 2) part += __shfl_xor(part, off);
+        const float kept = row.sum * keep;
+        row.sum = kept + part;
+        row.most = m2;
+        const float inverse = row.sum == 0.0f ? 0.0f : 1.0f / row.sum, weight = p * inverse;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) row.mean[c] *= kept * inverse;
+        const uint64_t any = __ballot(seen);
+        const uint64_t at = reinterpret_cast<uint64_t>(vr);
+        for (uint32_t y0 = 0; y0 < 64; y0 += 4) {
+            if (!((any >> y0) & 15u)) continue;
+            float value[4][4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const uint8_t* of = reinterpret_cast<const uint8_t*>(
+                        (uint64_t)__builtin_amdgcn_readlane((uint32_t)(at >> 32), y0 + y) << 32
+                        | (uint32_t)__builtin_amdgcn_readlane((uint32_t)at, y0 + y));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) value[y][c] = lane + 64 * c < D ? packed_element<DT>(of, lane + 64 * c) : 0.0f;
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                if (!((any >> (y0 + y)) & 1u)) continue;
+                const float of_all = as_f32(__builtin_amdgcn_readlane(as_u32(weight), y0 + y));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) row.mean[c] = __builtin_fmaf(of_all, value[y][c], row.mean[c]);
+            }
+        }
+    }
+    return row;
+}
+
+// One wave = one row of one head.  For head sizes of no whole tiles, pages of another size than whole tiles, and
+// as a check of the matrix cores' kernel: every row reads K and V for itself, bound by the latency of these reads
+// and by F32 arithmetic (24 prompts of up to 1201 rows, 32 / 4 heads of 64: 13 ms, 5 TFLOP/s, where the matrix cores
+// take 0.17 ms).
 template <int DT>
 __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedArgs a) {
     __shared__ float q_rows[4][kMaxPackedWidth];
-    const float inf = __builtin_inff();
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t s = blockIdx.z;
     const PackedSequence seq = packed_sequence(a, s);
@@ -79,92 +152,32 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
     const uint8_t* vb = a.v + hkv * a.v_head;
     const int32_t* pages = a.table.base ? a.table.row(s) : nullptr;
     const uint32_t row_tiles = a.d_tiles * kTile16;
-    // addresses of a token's rows; false: absent
-    auto token_rows = [&](uint32_t x, const uint8_t** kr, const uint8_t** vr) -> bool {
-        if (x >= seq.cached) {
-            const uint32_t t = seq.start + (x - seq.cached);
-            const uint64_t at = (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32;
-            *kr = kb + at;
-            *vr = vb + at;
-            return true;
-        }
-        const uint32_t slot = divided(x, a.page_rows, a.div_page_rows);
-        const uint32_t page = (uint32_t)pages[(uint64_t)(slot >> 4) * kTileSlots + (slot & 15u)];
-        if (page >= a.pages) return false;
-        const uint32_t r = x - slot * a.page_rows;
-        const uint64_t at = (uint64_t)(r >> 4) * row_tiles + (r & 15u) * 32;
-        *kr = a.k_pages + page * a.k_page + hkv * a.k_page_head + at;
-        *vr = a.v_pages + page * a.v_page + hkv * a.v_page_head + at;
-        return true;
-    };
-    auto element = [&](const uint8_t* row, uint32_t d) {
-        return wide16<DT>(*reinterpret_cast<const uint16_t*>(row + (d >> 4) * kTile16 + (d & 15u) * 2));
-    };
     for (uint32_t i = blockIdx.x * 4 + wave; i < rows; i += gridDim.x * 4) {
         const uint32_t t = seq.start + i;
-        const uint8_t* qr = a.q + head * a.q_head + (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32;
-        for (uint32_t d = lane; d < a.D; d += 64) q_rows[wave][d] = element(qr, d) * a.scale;
+        const uint64_t row_at = (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32;
+        const uint8_t* qr = a.q + head * a.q_head + row_at;
+        for (uint32_t d = lane; d < a.D; d += 64) q_rows[wave][d] = packed_element<DT>(qr, d) * a.scale;
         __builtin_amdgcn_wave_barrier();
         const uint32_t own = a.tree.base ? (a.tree.cols * 32 < seq.rows ? a.tree.cols * 32 : seq.rows) : i + 1;
-        const uint32_t tokens = seq.cached + own;
-        float m = -inf, sum = 0.0f, acc[4] = {0, 0, 0, 0};
-        for (uint32_t x0 = 0; x0 < tokens; x0 += 64) {
-            const uint32_t x = x0 + lane;
-            bool seen = x < tokens;
-            if (seen && x >= seq.cached && a.tree.base) {
-                const uint32_t j = x - seq.cached;
-                seen = ((uint32_t)a.tree.at(t, j >> 5) >> (j & 31u)) & 1u;
+        const PackedRow row = packed_row<DT>(a.D, q_rows[wave], seq.cached + own, vb + row_at,
+                                             [&](uint32_t x, const uint8_t** kr, const uint8_t** vr) -> bool {
+            if (x >= seq.cached) {
+                const uint32_t j = x - seq.cached, own_t = seq.start + j;
+                if (a.tree.base && !(((uint32_t)a.tree.at(t, j >> 5) >> (j & 31u)) & 1u)) return false;
+                const uint64_t at = (uint64_t)(own_t >> 4) * row_tiles + (own_t & 15u) * 32;
+                *kr = kb + at;
+                *vr = vb + at;
+                return true;
             }
-            // (a token that is not seen has the address of one that is there, the row's own)
-            const uint8_t *kr = nullptr, *vr = vb + (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32;
-            seen = seen && token_rows(x, &kr, &vr);
-            float score = -inf;
-            if (seen) {
-                score = 0.0f;
-                uint32_t d = 0;
-                for (; d + 8 <= a.D; d += 8) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(kr + (d >> 4) * kTile16 + (d & 15u) * 2);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        score = __builtin_fmaf(q_rows[wave][d + j], wide16<DT>(w[j >> 1] >> (16 * (j & 1)) & 0xFFFFu), score);
-                }
-                for (; d < a.D; ++d) score = __builtin_fmaf(q_rows[wave][d], element(kr, d), score);
-            }
-            float top = score;
-            for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
-            const float m2 = fmaxf(m, top);
-            const float base = m2 == -inf ? 0.0f : m2;
-            const float p = seen ? expf(score - base) : 0.0f;   // a NaN score stays one
-            const float keep = m == -inf ? 0.0f : expf(m - base);
-            float part = p;
-            for (int off = 1; off < 64; off *= 2) part += __shfl_xor(part, off);
-            sum = sum * keep + part;
-            m = m2;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] *= keep;
-            const uint64_t any = __ballot(seen);
-            const uint64_t at = reinterpret_cast<uint64_t>(vr);
-            for (uint32_t y0 = 0; y0 < 64; y0 += 4) {
-                if (!((any >> y0) & 15u)) continue;
-                float value[4][4];
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const uint8_t* of = reinterpret_cast<const uint8_t*>(
-                            (uint64_t)__builtin_amdgcn_readlane((uint32_t)(at >> 32), y0 + y) << 32
-                            | (uint32_t)__builtin_amdgcn_readlane((uint32_t)at, y0 + y));
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) value[y][c] = lane + 64 * c < a.D ? element(of, lane + 64 * c) : 0.0f;
-                }
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    if (!((any >> (y0 + y)) & 1u)) continue;
-                    const float py = as_f32(__builtin_amdgcn_readlane(as_u32(p), y0 + y));
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(py, value[y][c], acc[c]);
-                }
-            }
-        }
-        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const uint32_t slot = divided(x, a.page_rows, a.div_page_rows);
+            const uint32_t page = (uint32_t)pages[(uint64_t)(slot >> 4) * kTileSlots + (slot & 15u)];
+            if (page >= a.pages) return false;
+            const uint32_t r = x - slot * a.page_rows;
+            const uint64_t at = (uint64_t)(r >> 4) * row_tiles + (r & 15u) * 32;
+            *kr = a.k_pages + page * a.k_page + hkv * a.k_page_head + at;
+            *vr = a.v_pages + page * a.v_page + hkv * a.v_page_head + at;
+            return true;
+        });
         uint8_t* ob = a.out + (uint64_t)(t >> 4) * a.out_tile_cols * kTile16 + (t & 15u) * 32;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -172,7 +185,7 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
             if (d >= a.D) continue;
             const uint32_t col = head * a.D + d;
             *reinterpret_cast<uint16_t*>(ob + (uint64_t)(col >> 4) * kTile16 + (col & 15u) * 2) =
-                    (uint16_t)narrow2<DT>(sum == 0.0f ? 0.0f : acc[c] * inverse, 0.0f);
+                    (uint16_t)narrow2<DT>(row.sum == 0.0f ? 0.0f : row.mean[c], 0.0f);
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -197,6 +210,9 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // sum is taken of the unrounded ones.  F16 lifts p by 2^kLift so that small probabilities keep their
 // bits: they are at most 2^(kLift + kSlack), and subnormal below 2^-22 of the largest.
 //
+// The sums may pass F32's range where their mean does not (BF16's range is as wide): a row with a sum near its end is
+// taken again, as the other kernel does (near_end).
+//
 // Long prompts are bound by the matrix and the vector units, busy for 0.43 and 0.44 of the cycles (8191 rows,
 // 32 / 8 heads of 128 BF16: 583 us, 940 TFLOP/s of 1212 that a large product reaches); shorter ones wait
 // more (24 prompts of up to 1201 rows of 64: 174 us, 390 TFLOP/s); single tokens are bound by memory (32
@@ -210,6 +226,8 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // ---------------------------------------------------------------------------
 
 constexpr float kLowest = -3.4028234663852886e38f;
+// 2^115, as bits: four teams' and 512 pieces' sums of this size add up to less than the end of F32.
+constexpr uint32_t kNearEnd = (127u + 115u) << 23;
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -417,6 +435,123 @@ __device__ __forceinline__ PackedShare packed_share(const SdpaPackedArgs& a, uin
     return p;
 }
 
+// The block of rows that a workgroup takes (m_block .. of m_end rows times heads) and its token blocks.
+struct PackedBlock {
+    uint32_t s, hkv, pieces, m_block, m_end;
+    uint32_t own;                 // own rows that some row of the block sees
+    uint32_t begin, end;          // token blocks
+    PackedSequence seq;
+    PackedTiles tiles;
+};
+// false: there is none for this workgroup
+template <uint32_t BM, uint32_t NT>
+__device__ __forceinline__ bool packed_block(const SdpaPackedArgs& a, PackedBlock* p) {
+    uint32_t rb, piece = 0, size = 0;
+    p->pieces = 1;
+    if (a.places) {
+        const uint32_t index = divided(blockIdx.x, a.Hkv, a.div_hkv);
+        p->hkv = blockIdx.x - index * a.Hkv;
+        const PackedShare share = packed_share<BM, NT>(a, index, false);
+        if (share.s == ~0u) return false;
+        p->s = share.s; rb = share.row_block; piece = share.piece; p->pieces = share.pieces; size = share.size;
+        p->seq = share.seq;
+    } else {
+        // unit (sequence, KV head) fastest: consecutive workgroups go to different dies, a unit's row
+        // blocks to the same one where the units are a multiple of eight.  Late rows, which see the
+        // most, go first.
+        const uint32_t units = a.sequences * a.Hkv;
+        const uint32_t rb_up = divided(blockIdx.x, units, a.div_units), unit = blockIdx.x - rb_up * units;
+        rb = a.row_blocks - 1 - rb_up;
+        p->s = divided(unit, a.Hkv, a.div_hkv);
+        p->hkv = unit - p->s * a.Hkv;
+        p->seq = packed_sequence(a, p->s);
+    }
+    const uint32_t rows = p->seq.rows < a.max_rows ? p->seq.rows : a.max_rows;
+    p->m_end = rows * a.group;
+    p->m_block = rb * BM;
+    if (p->m_block >= p->m_end) return false;
+    if (a.tree.base) p->own = a.tree.cols * 32 < p->seq.rows ? a.tree.cols * 32 : p->seq.rows;
+    else {
+        const uint32_t m_last = p->m_block + BM < p->m_end ? p->m_block + BM - 1 : p->m_end - 1;
+        p->own = divided(m_last, a.group, a.div_group) + 1;
+    }
+    p->tiles.cached = p->seq.cached;
+    p->tiles.prefix = (p->seq.cached + 15) >> 4;
+    p->tiles.first = p->seq.start >> 4;
+    p->tiles.count = p->tiles.prefix + ((p->seq.start + p->own + 15) >> 4) - p->tiles.first;
+    const uint32_t blocks = (p->tiles.count + NT - 1) / NT;
+    p->begin = 0;
+    p->end = blocks;
+    if (p->pieces > 1) {
+        p->begin = piece * size;
+        p->end = p->begin + size < blocks ? p->begin + size : blocks;
+    }
+    return true;
+}
+
+// A row of the workgroup's block over the block's tokens once more, by one wave, and to its place; `q` is LDS of the
+// wave's own.  A function that is called, and finds out everything anew from the kernel's arguments: inlined, what this
+// (hardly ever taken) path needs is kept in registers through the main loop (prompts of heads of 64: 181 us instead
+// of 173).
+template <int DT, uint32_t BM, uint32_t NT>
+static __device__ __attribute__((noinline, cold)) void packed_again(const SdpaPackedArgs* args, float* q, uint32_t row_in_block) {
+    const SdpaPackedArgs& a = *args;
+    PackedBlock b;
+    if (!packed_block<BM, NT>(a, &b)) return;
+    const uint32_t m = b.m_block + row_in_block;
+    if (m >= b.m_end) return;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t i = divided(m, a.group, a.div_group), t = b.seq.start + i;
+    const uint32_t head = b.hkv * a.group + (m - i * a.group);
+    const uint32_t row_tiles = a.d_tiles * kTile16;
+    const uint64_t row_at = (uint64_t)(t >> 4) * row_tiles + (t & 15u) * 32;
+    const uint8_t* qr = a.q + head * a.q_head + row_at;
+    __builtin_amdgcn_wave_barrier();
+    for (uint32_t d = lane; d < a.D; d += 64) q[d] = packed_element<DT>(qr, d) * a.scale;
+    __builtin_amdgcn_wave_barrier();
+    const uint32_t visible = a.tree.base ? b.own : i + 1;
+    const uint8_t *kb = a.k + b.hkv * a.k_head, *vb = a.v + b.hkv * a.v_head;
+    const PackedRow row = packed_row<DT>(a.D, q, (b.end - b.begin) * NT * 16, vb + row_at,
+                                         [&](uint32_t n, const uint8_t** kr, const uint8_t** vr) -> bool {
+        const uint32_t x = b.begin * NT + (n >> 4), r = n & 15u;        // tile, row in it
+        if (x >= b.tiles.prefix) {
+            const uint32_t tile = b.tiles.first + x - b.tiles.prefix, j = tile * 16 + r - b.seq.start;
+            if (j >= visible) return false;                             // (rows before the first one wrap)
+            if (a.tree.base && !(((uint32_t)a.tree.at(t, j >> 5) >> (j & 31u)) & 1u)) return false;
+            *kr = kb + (uint64_t)tile * row_tiles + r * 32;
+            *vr = vb + (uint64_t)tile * row_tiles + r * 32;
+            return true;
+        }
+        if (x * 16 + r >= b.tiles.cached) return false;
+        const uint32_t slot = divided(x, a.page_tiles, a.div_page_tiles);
+        const uint32_t page = (uint32_t)a.table.at(b.s, slot);
+        if (page >= a.pages) return false;
+        const uint64_t at = (uint64_t)(x - slot * a.page_tiles) * row_tiles + r * 32;
+        *kr = a.k_pages + page * a.k_page + b.hkv * a.k_page_head + at;
+        *vr = a.v_pages + page * a.v_page + b.hkv * a.v_page_head + at;
+        return true;
+    });
+    // A part's sum of probabilities is brought to 2^-14 .. 2^-13 by a power of two, which its reference takes up:
+    // the unnormalised sums are then far from the end.
+    int32_t exponent = 0;
+    if (row.sum > 0.0f) exponent = (int32_t)(as_u32(row.sum) >> 23) - 126 + 13;
+    const float l = __builtin_ldexpf(row.sum, -exponent);
+    uint8_t* to = a.out + ((uint64_t)(t >> 4) * a.out_tile_cols + head * a.d_tiles) * kTile16 + (t & 15u) * 32;
+    const uint64_t part = (uint64_t)blockIdx.x * BM + row_in_block;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t d = lane + 64 * c;
+        if (d >= a.D) continue;
+        const float mean = row.sum == 0.0f ? 0.0f : row.mean[c];
+        if (b.pieces > 1) a.parts[part * a.D + d] = mean * l;
+        else *reinterpret_cast<uint16_t*>(to + (d >> 4) * kTile16 + (d & 15u) * 2) = (uint16_t)narrow2<DT>(mean, 0.0f);
+    }
+    if (b.pieces > 1 && lane == 0) {
+        a.part_stats[part * 2] = row.sum == 0.0f ? kLowest : row.most * 1.44269504088896340736f + (float)exponent;
+        a.part_stats[part * 2 + 1] = l;
+    }
+}
+
 // Waves per SIMD: as many workgroups as the stages leave room for in the LDS of a CU, up to two, or
 // three where the registers last (packed prompts of heads of 64 take 174 us with three and 207 us
 // with two).
@@ -440,52 +575,21 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     // knows that a read of one need not wait for the loader's writes to the other.
     __shared__ __attribute__((aligned(1024))) uint8_t k_even[WK][kStage], k_odd[WK][kStage];
     __shared__ __attribute__((aligned(1024))) uint8_t v_even[WK][kStage], v_odd[WK][kStage];
+    // For packed_again: the address of `a` (the one argument) waits in LDS, for where it is in registers the compiler reads
+    // the arguments again and again in the main loop instead of keeping them.
+    __shared__ float q_again[4][32 * KS];
+    __shared__ const SdpaPackedArgs* args_at;
+    args_at = (const SdpaPackedArgs*)__builtin_amdgcn_kernarg_segment_ptr();
     const uint32_t lane = threadIdx.x & 63u, column = Shape::column(lane);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t team = wave / WQ, member = wave % WQ;
 
-    uint32_t s, hkv, rb, piece = 0, pieces = 1, size = 0;
-    PackedSequence seq;
-    if (a.places) {
-        const uint32_t index = divided(blockIdx.x, a.Hkv, a.div_hkv);
-        hkv = blockIdx.x - index * a.Hkv;
-        const PackedShare share = packed_share<BM, NT>(a, index, false);
-        if (share.s == ~0u) return;
-        s = share.s; rb = share.row_block; piece = share.piece; pieces = share.pieces; size = share.size;
-        seq = share.seq;
-    } else {
-        // unit (sequence, KV head) fastest: consecutive workgroups go to different dies, a unit's row
-        // blocks to the same one where the units are a multiple of eight.  Late rows, which see the
-        // most, go first.
-        const uint32_t units = a.sequences * a.Hkv;
-        const uint32_t rb_up = divided(blockIdx.x, units, a.div_units), unit = blockIdx.x - rb_up * units;
-        rb = a.row_blocks - 1 - rb_up;
-        s = divided(unit, a.Hkv, a.div_hkv);
-        hkv = unit - s * a.Hkv;
-        seq = packed_sequence(a, s);
-    }
-    const uint32_t rows = seq.rows < a.max_rows ? seq.rows : a.max_rows;
-    const uint32_t m_end = rows * a.group, m_block = rb * BM;
-    if (m_block >= m_end) return;
-
-    // own rows that some row of the block sees
-    uint32_t own;
-    if (a.tree.base) own = a.tree.cols * 32 < seq.rows ? a.tree.cols * 32 : seq.rows;
-    else {
-        const uint32_t m_last = m_block + BM < m_end ? m_block + BM - 1 : m_end - 1;
-        own = divided(m_last, a.group, a.div_group) + 1;
-    }
-    PackedTiles tiles;
-    tiles.cached = seq.cached;
-    tiles.prefix = (seq.cached + 15) >> 4;
-    tiles.first = seq.start >> 4;
-    tiles.count = tiles.prefix + ((seq.start + own + 15) >> 4) - tiles.first;
-    const uint32_t blocks = (tiles.count + NT - 1) / NT;
-    uint32_t b_begin = 0, b_end = blocks;
-    if (pieces > 1) {
-        b_begin = piece * size;
-        b_end = b_begin + size < blocks ? b_begin + size : blocks;
-    }
+    PackedBlock block;
+    if (!packed_block<BM, NT>(a, &block)) return;
+    const uint32_t s = block.s, hkv = block.hkv, pieces = block.pieces, m_end = block.m_end, m_block = block.m_block;
+    const uint32_t b_begin = block.begin, b_end = block.end;
+    const PackedSequence seq = block.seq;
+    const PackedTiles tiles = block.tiles;
 
     // this wave's columns: rows of the sequence, and the wave's range of them
     const uint32_t m_wave = m_block + member * W * QT;
@@ -883,6 +987,23 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
 #pragma unroll
     for (int q = 0; q < QT; ++q) sum[q] = Shape::add(sum[q]);
 
+    // Columns with a sum near the end of F32 or past it, a bit each (a row whose probabilities' sum is a NaN is one in
+    // any case).
+    auto near_end = [&](int q) __attribute__((always_inline)) -> uint32_t {
+        if constexpr (DT != IOMX_DT_BF16) return 0u;
+        uint32_t most = 0;               // magnitudes in the order of their bits, a NaN above all
+#pragma unroll
+        for (int d = 0; d < Shape::kAccs; ++d)
+#pragma unroll
+            for (int j = 0; j < 4 * Shape::kAccQuads; ++j) {
+                const uint32_t size = as_u32(acc[d][q][j]) & 0x7FFFFFFFu;
+                most = most > size ? most : size;
+            }
+        const uint64_t lanes = __ballot(most >= kNearEnd && sum[q] == sum[q]);
+        const uint32_t columns = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+        return W == 32 ? columns : (columns | columns >> 16) & 0xFFFFu;
+    };
+
     // A row's place: its parts, or its first feature tile in the output (features of a head are whole
     // tiles).
     const uint64_t part = (uint64_t)blockIdx.x * BM;
@@ -902,7 +1023,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
             const uint32_t m = m_wave + W * q + column;
-            if (m >= m_end) continue;
+            if (m < m_end) {
             float* parts = pieces > 1 ? a.parts + (part + m - m_block) * a.D : nullptr;
             uint8_t* to = result_of(m);
 #pragma unroll
@@ -919,14 +1040,33 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
                 a.part_stats[(part + m - m_block) * 2] = ref[q];
                 a.part_stats[(part + m - m_block) * 2 + 1] = sum[q];
             }
+            }
+            // (over what was stored)
+            const uint32_t near = near_end(q);
+            if (near) __builtin_amdgcn_s_waitcnt(0);
+            for (uint32_t rest = near; rest; rest &= rest - 1)
+                packed_again<DT, BM, NT>(args_at, q_again[wave], member * W * QT + W * q + __ffs(rest) - 1);
         }
     } else {
         // The teams meet in LDS, a wave's columns at a time: a wave leaves its sums scaled to the
         // largest reference of all teams.
         constexpr uint32_t kFeatures = 32 * KS, kRows = 16;
         __shared__ float meet_ref[WK][BM], meet_sum[WK][BM];
+        __shared__ uint32_t meet_near[WK][BM / W];
         static_assert(WK * kRows * kFeatures * 4 <= WK * kStage, "the teams' sums fit a stage of K");
         float* meet = reinterpret_cast<float*>(&k_even[0][0]);     // [team][row][feature]
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            const uint32_t near = near_end(q);
+            if (lane == 0) meet_near[team][member * QT + q] = near;
+        }
+        // (after the first barrier) a column tile's rows that are taken again
+        auto near_of = [&](uint32_t column_tile) __attribute__((always_inline)) -> uint32_t {
+            uint32_t near = 0;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) near |= meet_near[w][column_tile];
+            return near;
+        };
         if (lane < W) {
 #pragma unroll
             for (int q = 0; q < QT; ++q) {
@@ -957,7 +1097,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
             __syncthreads();
             for (uint32_t i = threadIdx.x; i < kRows * kFeatures / 4; i += 256) {
                 const uint32_t row = i / (kFeatures / 4), feature = i % (kFeatures / 4) * 4, m = turn * kRows + row;
-                if (m_block + m >= m_end || feature >= a.D) continue;
+                if (m_block + m >= m_end || feature >= a.D || ((near_of(m / W) >> (m % W)) & 1u)) continue;
                 float top = kLowest, l = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WK; ++w) top = fmaxf(top, meet_ref[w][m]);
@@ -977,6 +1117,11 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
                     *reinterpret_cast<u32x2*>(result_of(m_block + m) + (feature >> 4) * kTile16 + (feature & 15u) * 2) = finished(o, l);
             }
         }
+        // the waves take these rows in turn
+        uint32_t turn = 0;
+        for (uint32_t n = 0; n < BM / W; ++n)
+            for (uint32_t rest = near_of(n); rest; rest &= rest - 1)
+                if (turn++ % 4 == wave) packed_again<DT, BM, NT>(args_at, q_again[wave], n * W + __ffs(rest) - 1);
     }
 }
 
