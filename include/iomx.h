@@ -430,8 +430,10 @@ int iomx_launch_softmax(const iomx_softmax_desc* desc, iomx_stream_t stream);
  *
  * BF16 and F16, any head size up to 256.  Scores, softmax statistics and sums are F32, the
  * unnormalised probabilities are rounded to the leaf on the matrix cores, one rounding at
- * the store.  A row that sees nothing, or only scores of -inf, is +0; one that sees a NaN
- * or a score of +inf is NaN.  Rows of no sequence are left as they were; `max_rows` is the
+ * the store.  A row that sees nothing, or only scores of -inf, is +0; one that sees a score
+ * of NaN or +inf is NaN.  Values of any size give their weighted mean where it is finite; an
+ * infinite value that a row sees is that feature's result however small its probability
+ * (a NaN where there are both signs, or a NaN).  Rows of no sequence are left as they were; `max_rows` is the
  * caller's bound on starts[s+1] - starts[s], and rows past it are left as they were too (the
  * launch has workgroups for max_rows rows of every sequence: a tight bound, 1 in a step of
  * single tokens, picks the right kernel).

@@ -73,15 +73,19 @@ struct PackedRow {
 
 // One row: 64 tokens at a time, a lane forms the score of one token, then the lanes take the features, four
 // tokens' values on their way together (with eight, 15.4 ms instead of 13.1 for the prompts below).  Running maximum,
-// sum and mean (a sum of values may pass F32's range where their mean does not); everything in F32.
+// sum and mean (a sum of values may pass F32's range where their mean does not); everything in F32.  `apart` keeps the
+// values apart that are not finite: an infinity shows however small its probability, also where that is zero in F32
+// (not done before a mean has come out that is not finite: 4 prompts of up to 300 rows, 8 / 2 heads of 40, would take
+// 184 us instead of 131).
 // `q` is the row times 1 / sqrt(D), in LDS.  locate(n, &k_row, &v_row) says whether the row sees token n and where
 // it lies; `there` is the address of any row (read, and not used, for a token that is not seen).
 template <int DT, class Locate>
 __device__ __forceinline__ PackedRow packed_row(uint32_t D, const float* q, uint32_t tokens, const uint8_t* there,
-                                                const Locate& locate) {
+                                                bool apart, const Locate& locate) {
     const float inf = __builtin_inff();
     const uint32_t lane = threadIdx.x & 63u;
     PackedRow row = {-inf, 0.0f, {0, 0, 0, 0}};
+    float wild[4] = {0, 0, 0, 0};
     for (uint32_t n0 = 0; n0 < tokens; n0 += 64) {
         const uint8_t *kr = nullptr, *vr = there;
         const bool seen = n0 + lane < tokens && locate(n0 + lane, &kr, &vr);
@@ -124,6 +128,16 @@ __device__ __forceinline__ PackedRow packed_row(uint32_t D, const float* q, uint
 #pragma unroll
                 for (int c = 0; c < 4; ++c) value[y][c] = lane + 64 * c < D ? packed_element<DT>(of, lane + 64 * c) : 0.0f;
             }
+            if (apart) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (fabsf(value[y][c]) < inf) continue;
+                        if ((any >> (y0 + y)) & 1u) wild[c] += value[y][c];
+                        value[y][c] = 0.0f;
+                    }
+            }
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
                 if (!((any >> (y0 + y)) & 1u)) continue;
@@ -133,6 +147,9 @@ __device__ __forceinline__ PackedRow packed_row(uint32_t D, const float* q, uint
             }
         }
     }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (wild[c] != 0.0f) row.mean[c] += wild[c];
     return row;
 }
 
@@ -159,8 +176,7 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
         for (uint32_t d = lane; d < a.D; d += 64) q_rows[wave][d] = packed_element<DT>(qr, d) * a.scale;
         __builtin_amdgcn_wave_barrier();
         const uint32_t own = a.tree.base ? (a.tree.cols * 32 < seq.rows ? a.tree.cols * 32 : seq.rows) : i + 1;
-        const PackedRow row = packed_row<DT>(a.D, q_rows[wave], seq.cached + own, vb + row_at,
-                                             [&](uint32_t x, const uint8_t** kr, const uint8_t** vr) -> bool {
+        auto locate = [&](uint32_t x, const uint8_t** kr, const uint8_t** vr) -> bool {
             if (x >= seq.cached) {
                 const uint32_t j = x - seq.cached, own_t = seq.start + j;
                 if (a.tree.base && !(((uint32_t)a.tree.at(t, j >> 5) >> (j & 31u)) & 1u)) return false;
@@ -177,7 +193,15 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
             *kr = a.k_pages + page * a.k_page + hkv * a.k_page_head + at;
             *vr = a.v_pages + page * a.v_page + hkv * a.v_page_head + at;
             return true;
-        });
+        };
+        PackedRow row;
+        for (bool apart = false;; apart = true) {
+            row = packed_row<DT>(a.D, q_rows[wave], seq.cached + own, vb + row_at, apart, locate);
+            bool finite = true;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) finite = finite && fabsf(row.mean[c]) < __builtin_inff();
+            if (apart || row.sum != row.sum || __all(finite)) break;
+        }
         uint8_t* ob = a.out + (uint64_t)(t >> 4) * a.out_tile_cols * kTile16 + (t & 15u) * 32;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -210,8 +234,9 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // sum is taken of the unrounded ones.  F16 lifts p by 2^kLift so that small probabilities keep their
 // bits: they are at most 2^(kLift + kSlack), and subnormal below 2^-22 of the largest.
 //
-// The sums may pass F32's range where their mean does not (BF16's range is as wide): a row with a sum near its end is
-// taken again, as the other kernel does (near_end).
+// The sums may pass F32's range where their mean does not (BF16's range is as wide), and an infinite value meets
+// probabilities of zero: a row with a sum near the range's end or past it is taken again, as the other kernel does
+// (near_end).
 //
 // Long prompts are bound by the matrix and the vector units, busy for 0.43 and 0.44 of the cycles (8191 rows,
 // 32 / 8 heads of 128 BF16: 583 us, 940 TFLOP/s of 1212 that a large product reaches); shorter ones wait
@@ -511,7 +536,7 @@ static __device__ __attribute__((noinline, cold)) void packed_again(const SdpaPa
     __builtin_amdgcn_wave_barrier();
     const uint32_t visible = a.tree.base ? b.own : i + 1;
     const uint8_t *kb = a.k + b.hkv * a.k_head, *vb = a.v + b.hkv * a.v_head;
-    const PackedRow row = packed_row<DT>(a.D, q, (b.end - b.begin) * NT * 16, vb + row_at,
+    const PackedRow row = packed_row<DT>(a.D, q, (b.end - b.begin) * NT * 16, vb + row_at, true,
                                          [&](uint32_t n, const uint8_t** kr, const uint8_t** vr) -> bool {
         const uint32_t x = b.begin * NT + (n >> 4), r = n & 15u;        // tile, row in it
         if (x >= b.tiles.prefix) {
@@ -531,8 +556,8 @@ static __device__ __attribute__((noinline, cold)) void packed_again(const SdpaPa
         *vr = a.v_pages + page * a.v_page + b.hkv * a.v_page_head + at;
         return true;
     });
-    // A part's sum of probabilities is brought to 2^-14 .. 2^-13 by a power of two, which its reference takes up:
-    // the unnormalised sums are then far from the end.
+    // A part's sum of probabilities is brought to 2^-14 .. 2^-13 by a power of two, which its reference takes up (next to
+    // the 2^kLift that the other parts' sums hold): the unnormalised sums are then far from the end.
     int32_t exponent = 0;
     if (row.sum > 0.0f) exponent = (int32_t)(as_u32(row.sum) >> 23) - 126 + 13;
     const float l = __builtin_ldexpf(row.sum, -exponent);
@@ -542,12 +567,12 @@ static __device__ __attribute__((noinline, cold)) void packed_again(const SdpaPa
     for (int c = 0; c < 4; ++c) {
         const uint32_t d = lane + 64 * c;
         if (d >= a.D) continue;
-        const float mean = row.sum == 0.0f ? 0.0f : row.mean[c];
-        if (b.pieces > 1) a.parts[part * a.D + d] = mean * l;
-        else *reinterpret_cast<uint16_t*>(to + (d >> 4) * kTile16 + (d & 15u) * 2) = (uint16_t)narrow2<DT>(mean, 0.0f);
+        const float mean = row.mean[c];
+        if (b.pieces > 1) a.parts[part * a.D + d] = row.sum == 0.0f ? mean : mean * l;
+        else *reinterpret_cast<uint16_t*>(to + (d >> 4) * kTile16 + (d & 15u) * 2) = (uint16_t)narrow2<DT>(row.sum == 0.0f ? 0.0f : mean, 0.0f);
     }
     if (b.pieces > 1 && lane == 0) {
-        a.part_stats[part * 2] = row.sum == 0.0f ? kLowest : row.most * 1.44269504088896340736f + (float)exponent;
+        a.part_stats[part * 2] = row.sum == 0.0f ? kLowest : row.most * 1.44269504088896340736f + (float)exponent + PackedLeaf<DT>::kLift;
         a.part_stats[part * 2 + 1] = l;
     }
 }
@@ -990,7 +1015,6 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
     // Columns with a sum near the end of F32 or past it, a bit each (a row whose probabilities' sum is a NaN is one in
     // any case).
     auto near_end = [&](int q) __attribute__((always_inline)) -> uint32_t {
-        if constexpr (DT != IOMX_DT_BF16) return 0u;
         uint32_t most = 0;               // magnitudes in the order of their bits, a NaN above all
 #pragma unroll
         for (int d = 0; d < Shape::kAccs; ++d)
@@ -1169,7 +1193,9 @@ __global__ __launch_bounds__(256) void sdpa_packed_join_kernel(const SdpaPackedA
             if (p0 + n >= share.pieces) break;
             const float factor = __builtin_amdgcn_exp2f(ref[n] - r);
             l += sum[n] * factor;
-            o += part[n] * factor;
+            // (an infinite value shows whatever its part's weight)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += fabsf(part[n][j]) < __builtin_inff() ? part[n][j] * factor : part[n][j];
         }
     }
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
