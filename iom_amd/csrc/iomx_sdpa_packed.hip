@@ -1246,6 +1246,8 @@ int sdpa_packed_request(int dtype, const iomx_view* q, const iomx_view* k, const
     // rows times heads of a KV head are counted in 32 bits
     uint64_t paired;
     if (width > 0x7FFFFFF0ull || mul_overflows(qm.rows, Hq, &paired) || paired > 0x7FFFFFF0ull) return IOMX_ERR_OVERFLOW;
+    // and the tokens of a sequence, 64 at a time
+    if ((cached ? (uint64_t)a->table.cols * k_pages->dims[2] : 0) + qm.rows > 0xFFFFFF00ull) return IOMX_ERR_OVERFLOW;
     uint8_t* base = nullptr;
     uint64_t strides[2];
     plane_bytes_of(*q, 16, &base, &a->q_head);
