@@ -433,13 +433,15 @@ int iomx_launch_softmax(const iomx_softmax_desc* desc, iomx_stream_t stream);
  * the store.  A row that sees nothing, or only scores of -inf, is +0; one that sees a score
  * of NaN or +inf is NaN.  Values of any size give their weighted mean where it is finite; an
  * infinite value that a row sees is that feature's result however small its probability
- * (a NaN where there are both signs, or a NaN).  Rows of no sequence are left as they were; `max_rows` is the
- * caller's bound on starts[s+1] - starts[s], and rows past it are left as they were too (the
- * launch has workgroups for max_rows rows of every sequence: a tight bound, 1 in a step of
- * single tokens, picks the right kernel).
+ * (a NaN where there are both signs, or a NaN).  (On the matrix cores a row whose
+ * unnormalised sums pass 2^115, with values of about 1e28 and more, or are not finite is
+ * computed again on its own and costs up to some 300 times as much.)  Rows of no sequence are left
+ * as they were; `max_rows` is the caller's bound on starts[s+1] - starts[s], and rows past
+ * it are left as they were too (the launch has workgroups for max_rows rows of every
+ * sequence: a tight bound, 1 in a step of single tokens, picks the right kernel).
  *
- * path 0 picks the kernel: the matrix cores where D % 16 == 0, D <= 128 and P % 16 == 0,
- * else one wave per row and head; path 1 forces the latter (tests).
+ * path 0 picks the kernel: the matrix cores where D % 16 == 0 and P % 16 == 0 (or there
+ * are no pages), else one wave per row and head; path 1 forces the latter (tests).
  *
  * iomx_sdpa_packed_workspace gives the bytes and the alignment of the workspace that the
  * launch needs for these operands ({0, 1}: none); its contents need not be kept or cleared
@@ -472,7 +474,8 @@ int iomx_launch_rope_packed(int dtype, const iomx_view* x, const iomx_view* out,
  * source row is rows[e] of the I32 view `rows` [1,E] (the accepted ones of a drafted tree,
  * say; a number outside [0,T) skips its entry), or e itself where `rows` is null (E = T).
  * Any leaf, raw bits, D a multiple of 16.  Entries whose page is absent or past the table
- * are skipped.  Two entries that land on one slot leave either one's row there.
+ * are skipped.  Two entries that land on one slot (a page that two sequences share) leave a
+ * mixture of both rows there.
  */
 int iomx_launch_cache_append_packed(int dtype, const iomx_view* k, const iomx_view* v, const iomx_view* k_pages,
                                     const iomx_view* v_pages, const iomx_view* starts, const iomx_view* table,

@@ -37,7 +37,7 @@ struct LogprobsArgs {
 // product with log2 e taken from another: logits near the ends of the range stay finite), 64,
 // 32 or 16 logits at a time with the maximum moved before each, and the maximum of every cell (a group
 // of 64 to 256 columns, or a few groups) goes to the workspace.  2047 rows of 128256 BF16: 102 us, 5.1
-// TB/s, what a read of as many bytes reaches; the vector units are busy for two thirds of it.
+// TB/s, where a bare read reaches 6.6; the vector units are busy for two thirds of it.
 //
 // token_logprobs_finish, one wave per row (or four), joins the sums and picks the most likely tokens without
 // another pass: a value that K cells' maxima reach is reached by K logits, so only the cells that

@@ -239,9 +239,10 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // (near_end).
 //
 // Long prompts are bound by the matrix and the vector units, busy for 0.43 and 0.44 of the cycles (8191 rows,
-// 32 / 8 heads of 128 BF16: 583 us, 940 TFLOP/s of 1212 that a large product reaches); shorter ones wait
-// more (24 prompts of up to 1201 rows of 64: 174 us, 390 TFLOP/s); single tokens are bound by memory (32
-// tokens over 700 to 15001 cached ones, 8 KV heads of 128: 194 us, 5.2 TB/s).
+// 32 / 8 heads of 128 BF16: 565 to 600 us on different cards, 920 to 970 TFLOP/s, where library products of 4096^3
+// to 16384^3 reach 1163 to 1337); shorter ones wait more (24 prompts of up to 1201 rows of 64: 170 us, 400
+// TFLOP/s); single tokens are bound by memory (32 tokens over 700 to 15001 cached ones, 8 KV heads of 128: 195 us,
+// 5.2 TB/s, where a bare read reaches 6.6).
 //
 // Only blocks that a row does not see in full (the ends of the cached prefix, the diagonal, trees,
 // absent pages) form masks.  There V is cleared where no row may see it, and a value left that is
@@ -517,7 +518,8 @@ __device__ __forceinline__ bool packed_block(const SdpaPackedArgs& a, PackedBloc
 // A row of the workgroup's block over the block's tokens once more, by one wave, and to its place; `q` is LDS of the
 // wave's own.  A function that is called, and finds out everything anew from the kernel's arguments: inlined, what this
 // (hardly ever taken) path needs is kept in registers through the main loop (prompts of heads of 64: 181 us instead
-// of 173).
+// of 173).  It reads K and V for every row: where all values are 1e38, 4096 rows of 32 / 8 heads of 128 take 50 ms
+// instead of 0.18, 32 single tokens over 700 to 15001 cached ones 5.8 ms instead of 0.2.
 template <int DT, uint32_t BM, uint32_t NT>
 static __device__ __attribute__((noinline, cold)) void packed_again(const SdpaPackedArgs* args, float* q, uint32_t row_in_block) {
     const SdpaPackedArgs& a = *args;
@@ -578,7 +580,7 @@ static __device__ __attribute__((noinline, cold)) void packed_again(const SdpaPa
 }
 
 // Waves per SIMD: as many workgroups as the stages leave room for in the LDS of a CU, up to two, or
-// three where the registers last (packed prompts of heads of 64 take 174 us with three and 207 us
+// three where the registers last (packed prompts of heads of 64 take 169 us with three and 216 us
 // with two).
 constexpr int packed_waves(int KS, int WQ, int NT) {
     const int fit = 160 * 1024 / (4 * (4 / WQ) * NT * KS * 1024 + 2048), most = KS <= 2 && WQ == 4 ? 3 : 2;
@@ -1151,7 +1153,7 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
 
 // Joins the rows of a sequence and KV head whose tokens were shared out: a lane takes four features of
 // a row, and scales each part from its own reference.  Bound by the chain of reads that finds the
-// shares and then the parts: 7 us for 32 tokens, 9.4 us for eight trees of up to 61 rows (32 / 8 heads of 128).
+// shares and then the parts: 7.3 us for 32 tokens, 9.8 us for eight trees of up to 61 rows (32 / 8 heads of 128).
 template <int DT, uint32_t BM, uint32_t NT>
 __global__ __launch_bounds__(256) void sdpa_packed_join_kernel(const SdpaPackedArgs a) {
     const uint32_t chunks = a.D / 4;
