@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // (near_end).
 //
 // Long prompts are bound by the matrix and the vector units, busy for 0.43 and 0.44 of the cycles (8191 rows,
-// 32 / 8 heads of 128 BF16: 565 to 600 us on different cards, 920 to 970 TFLOP/s, where library products of 4096^3
+// 32 / 8 heads of 128 BF16: 565 to 610 us on different cards, 900 to 970 TFLOP/s, where library products of 4096^3
 // to 16384^3 reach 1163 to 1337); shorter ones wait more (24 prompts of up to 1201 rows of 64: 170 us, 400
 // TFLOP/s); single tokens are bound by memory (32 tokens over 700 to 15001 cached ones, 8 KV heads of 128: 195 us,
 // 5.2 TB/s, where a bare read reaches 6.6).
@@ -252,7 +252,8 @@ __global__ __launch_bounds__(256) void sdpa_packed_rows_kernel(const SdpaPackedA
 // ---------------------------------------------------------------------------
 
 constexpr float kLowest = -3.4028234663852886e38f;
-// 2^115, as bits: four teams' and 512 pieces' sums of this size add up to less than the end of F32.
+// 2^115, as bits: four teams' sums of this size and those of 1536 pieces (three for each of fewer than kPackedGroups
+// row blocks at the most, see packed_room) add up to less than 2^127.6.
 constexpr uint32_t kNearEnd = (127u + 115u) << 23;
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -1050,22 +1051,22 @@ __global__ __launch_bounds__(256, packed_waves(KS, WQ, NT)) void sdpa_packed_mfm
         for (int q = 0; q < QT; ++q) {
             const uint32_t m = m_wave + W * q + column;
             if (m < m_end) {
-            float* parts = pieces > 1 ? a.parts + (part + m - m_block) * a.D : nullptr;
-            uint8_t* to = result_of(m);
+                float* parts = pieces > 1 ? a.parts + (part + m - m_block) * a.D : nullptr;
+                uint8_t* to = result_of(m);
 #pragma unroll
-            for (int d = 0; d < Shape::kAccs; ++d)
+                for (int d = 0; d < Shape::kAccs; ++d)
 #pragma unroll
-                for (int u = 0; u < Shape::kAccQuads; ++u) {
-                    const uint32_t feature = Shape::feature(d, u, lane);
-                    if (feature >= a.D) continue;
-                    const f32x4_t o = quad_of(acc[d][q], u);
-                    if (parts) *reinterpret_cast<f32x4_t*>(parts + feature) = o;
-                    else *reinterpret_cast<u32x2*>(to + (feature >> 4) * kTile16 + (feature & 15u) * 2) = finished(o, sum[q]);
+                    for (int u = 0; u < Shape::kAccQuads; ++u) {
+                        const uint32_t feature = Shape::feature(d, u, lane);
+                        if (feature >= a.D) continue;
+                        const f32x4_t o = quad_of(acc[d][q], u);
+                        if (parts) *reinterpret_cast<f32x4_t*>(parts + feature) = o;
+                        else *reinterpret_cast<u32x2*>(to + (feature >> 4) * kTile16 + (feature & 15u) * 2) = finished(o, sum[q]);
+                    }
+                if (parts && lane < W) {
+                    a.part_stats[(part + m - m_block) * 2] = ref[q];
+                    a.part_stats[(part + m - m_block) * 2 + 1] = sum[q];
                 }
-            if (parts && lane < W) {
-                a.part_stats[(part + m - m_block) * 2] = ref[q];
-                a.part_stats[(part + m - m_block) * 2 + 1] = sum[q];
-            }
             }
             // (over what was stored)
             const uint32_t near = near_end(q);
