@@ -60,3 +60,33 @@ def test_large_values_of_either_sign(tree):
     case = Attention(62, BF16, (4, 2), 64, 16, [150, 20], [0, 0], cache=False, tree=tree, scale=0.5)
     with_values(case, lambda v: np.clip(v, -3, 3) * 1e38)
     assert np.isfinite(both(case)).all()
+
+
+@pytest.mark.parametrize("rows,ctx", [([1, 2], [2300, 40]), ([90, 7], [30, 0])])
+def test_a_recorded_step_with_large_values(rows, ctx):
+    """Rows that are taken again in a replayed graph: ordinary and large values in turn, each as the eager call."""
+    cases = [Attention(65, BF16, (8, 2), 64, 16, rows, ctx) for _ in range(2)]
+    with_values(cases[0], lambda v: np.clip(np.abs(v) + 0.25, 0.25, 2.0) * 1e38)
+    t = cases[0].upload()
+    views = {n: x.view() for n, x in t.items()}
+    rc, nbytes, _ = iomx.sdpa_packed_workspace(max_rows=cases[0].max_rows, **views)
+    iomx.check(rc)
+    ws = iomx.Buffer(nbytes) if nbytes else None
+    st = iomx.Stream()
+    iomx.synchronize()
+    st.begin_capture()
+    rc = iomx.sdpa_packed(max_rows=cases[0].max_rows, workspace=ws, stream=st, **views)
+    graph = st.end_capture()
+    iomx.check(rc)
+    for case in (cases[0], cases[1], cases[0], cases[1], cases[0]):
+        for name in ("v", "v_pages"):
+            t[name].view().from_host(getattr(case, name))
+        t["out"].buf.fill(0x5A)
+        iomx.synchronize()
+        graph.launch(st)
+        st.synchronize()
+        got = t["out"].view().to_host()
+        case.check(got)
+        assert np.array_equal(got, case.run())
+    graph.close()
+    st.close()
